@@ -124,6 +124,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                    c_vp]),
     "hl_argmax": (c_int, [c_vp, c_i64, c_int, c_int, c_vp, c_vp]),
     "hl_argmax_shard": (c_int, [c_vp, c_i64, c_int, c_int, c_i64, c_vp, c_vp, c_vp]),
+    "hl_extend_block_tables": (c_int, [c_vp, c_vp, c_int, c_vp, c_i64, c_int, c_vp, c_i64, c_int, c_i64, c_vp, c_vp,
+                                       c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "hl_store_kv_fp8_blocks": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int,
+                                       c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_i64, c_vp]),
+    "hl_paged_decode_fp8_blocks_workspace_size": (c_i64, [c_int, c_int, c_int]),
+    "hl_paged_decode_fp8_blocks": (c_int, [c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_vp, c_int, c_int,
+                                           c_int, c_int, c_int, c_int, c_i64, c_f32, c_vp, c_i64, c_vp, c_i64, c_vp]),
+    "hl_token_logprobs": (c_int, [c_vp, c_int, c_i64, c_i64, c_int, c_vp, c_int, c_vp, c_vp, c_vp, c_vp, c_vp]),
 }
 
 

@@ -30,6 +30,10 @@ SOURCES = [
     "pack_decode.cu",
     "layer_ops.cu",
     "allreduce.cu",
+    "page_tables.cu",
+    "store_kv_blocks.cu",
+    "paged_decode_blocks.cu",
+    "logprobs.cu",
 ]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

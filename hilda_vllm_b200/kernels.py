@@ -429,3 +429,167 @@ def argmax_shard(logits: torch.Tensor, index_offset: int, out_tokens: torch.Tens
     lib = _lib.load()
     check(lib.hl_argmax_shard(logits.data_ptr(), logits.stride(0), rows, vocab, int(index_offset),
                               out_tokens.data_ptr(), out_values.data_ptr(), _stream(logits)), "hl_argmax_shard")
+
+
+# ------------------------------------------------------------------------ page tables
+def _on_one_device(first: torch.Tensor, *rest: torch.Tensor) -> None:
+    """All tensors (None allowed) on one CUDA device."""
+    _cuda(first, *rest)
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+
+
+def _launch(name: str, t: torch.Tensor, *args) -> None:
+    """Calls the C entry point `name` on t's device, current or not, and that device's stream."""
+    fn = getattr(_lib.load(), name)
+    if t.get_device() == torch.cuda.current_device():
+        check(fn(*args, _stream(t)), name)
+    else:
+        with torch.cuda.device(t.device):
+            check(fn(*args, _stream(t)), name)
+
+
+def extend_block_tables(block_tables: torch.Tensor, cached_lens: torch.Tensor | None, query_lens: torch.Tensor,
+                        free_blocks: torch.Tensor, block_size: int, max_tokens: int) -> dict:
+    """Gives every sequence the pages its new tokens need and builds the batch description on the
+    device (hl_extend_block_tables): prefill_metadata without the host loop, for lengths and a free
+    list that are on the GPU.
+
+    block_tables [B, MB] int32, updated in place: row b keeps its ceil(cached_lens[b] / block_size)
+    first entries, takes the next ids of free_blocks [F] int32 for the others it needs, -1 behind
+    them.  cached_lens / query_lens [B] int32 (cached_lens None: all 0).  Returns the keys of
+    prefill_metadata (block_tables, cu_seqlens_q, cu_seqlens_k, positions int64 and slot_mapping of
+    max_tokens entries, 0 / -1 behind the batch's last token) plus context_lens and status, int32
+    [2]: pages taken, error bits (1: free list too short, 2: table too narrow, 4: more than
+    max_tokens tokens; what did not fit is -1)."""
+    _on_one_device(block_tables, cached_lens, query_lens, free_blocks)
+    b, width = block_tables.shape
+    assert block_tables.dtype == torch.int32 and block_tables.stride(1) == 1
+    assert query_lens.dtype == torch.int32 and query_lens.is_contiguous() and query_lens.shape == (b,)
+    if cached_lens is not None:
+        assert cached_lens.dtype == torch.int32 and cached_lens.is_contiguous() and cached_lens.shape == (b,)
+    assert free_blocks.dtype == torch.int32 and free_blocks.is_contiguous() and free_blocks.dim() == 1
+    dev = block_tables.device
+    cu_q = torch.empty(b + 1, dtype=torch.int32, device=dev)
+    cu_k = torch.empty(b + 1, dtype=torch.int32, device=dev)
+    context = torch.empty(b, dtype=torch.int32, device=dev)
+    positions = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    slots = torch.empty(max_tokens, dtype=torch.int32, device=dev)
+    status = torch.empty(2, dtype=torch.int32, device=dev)
+    _launch(
+        "hl_extend_block_tables", block_tables, _p(cached_lens), query_lens.data_ptr(), b, block_tables.data_ptr(),
+        block_tables.stride(0), width, free_blocks.data_ptr(), free_blocks.numel(), int(block_size), int(max_tokens),
+        cu_q.data_ptr(), cu_k.data_ptr(), context.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+        status.data_ptr())
+    return {"block_tables": block_tables, "cu_seqlens_q": cu_q, "cu_seqlens_k": cu_k, "context_lens": context,
+            "positions": positions, "slot_mapping": slots, "status": status}
+
+
+# ------------------------------------------------------------------------ block-scaled 8-bit cache
+def _check_block_cache(k_cache, v_cache, k_scales, v_scales):
+    """(num_blocks, block_size, Hk, D, scale_block) of a block-scaled cache."""
+    nb, bs, hk, d = k_cache.shape
+    assert k_cache.dtype == torch.float8_e4m3fn and v_cache.dtype == torch.float8_e4m3fn
+    assert k_cache.is_contiguous() and v_cache.is_contiguous() and v_cache.shape == k_cache.shape
+    assert k_scales.dtype == torch.float32 and v_scales.dtype == torch.float32
+    assert k_scales.is_contiguous() and v_scales.is_contiguous() and v_scales.shape == k_scales.shape
+    groups = k_scales.shape[1]
+    assert k_scales.shape == (nb, groups, hk) and groups > 0 and bs % groups == 0
+    return nb, bs, hk, d, bs // groups
+
+
+def store_kvcache_fp8_blocks(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                             k_scales: torch.Tensor, v_scales: torch.Tensor, block_tables: torch.Tensor,
+                             context_lens: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None) -> None:
+    """Stores new tokens into an 8-bit cache whose scales follow the data: one power of two per block
+    of tokens and head (hl_store_kv_fp8_blocks).
+
+    key/value [N, Hk, D] bf16 (row-strided views allowed); caches [NB, BS, Hk, D] e4m3; scales
+    [NB, BS / T, Hk] fp32, T a multiple of 64; block_tables [B, MB] int32; context_lens [B] int32
+    including the new tokens; cu_seqlens_q [B + 1] int32, the rows of each sequence (None: one row
+    per sequence).  Tokens that a block held before are rescaled when its scale grows; whatever a
+    page held for an earlier owner does not count."""
+    _on_one_device(key, value, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, cu_seqlens_q)
+    n, hk, hd = key.shape
+    nb, bs, hk2, hd2, t = _check_block_cache(k_cache, v_cache, k_scales, v_scales)
+    assert value.shape == key.shape and (hk, hd) == (hk2, hd2)
+    assert key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16
+    assert n == 0 or (key.stride(2) == 1 and value.stride(2) == 1 and key.stride(1) == hd and value.stride(1) == hd)
+    assert block_tables.dtype == torch.int32 and block_tables.stride(1) == 1
+    assert context_lens.dtype == torch.int32 and context_lens.is_contiguous()
+    b = context_lens.numel()
+    assert block_tables.shape[0] >= b
+    if cu_seqlens_q is not None:
+        assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.numel() == b + 1
+    # One row may come with any row stride (a slice of a single-row tensor).
+    krs, vrs = (key.stride(0), value.stride(0)) if n > 1 else (hk * hd, hk * hd)
+    _launch(
+        "hl_store_kv_fp8_blocks", key, key.data_ptr(), value.data_ptr(), krs, vrs, n, k_cache.data_ptr(),
+        v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
+        block_tables.shape[1], context_lens.data_ptr(), _p(cu_seqlens_q), b, hk, hd, bs, t, nb)
+
+
+def make_block_decode_workspace(batch: int, num_q_heads: int, num_kv_heads: int, device) -> torch.Tensor:
+    """Zero-filled workspace for paged_decode_fp8_blocks; serves every batch up to `batch`."""
+    n = _lib.load().hl_paged_decode_fp8_blocks_workspace_size(batch, num_q_heads, num_kv_heads)
+    if n < 0:
+        raise ValueError("bad decode workspace shape")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def paged_decode_fp8_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                            v_scales: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                            softmax_scale: float, out: torch.Tensor | None = None,
+                            workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_decode over the cache of store_kvcache_fp8_blocks: one new token per sequence, q
+    [B, Hq, D] (or [B, 1, Hq, D]) bf16, Hq / Hk <= 16; block_tables [>= B, MB] int32, context_lens
+    [>= B] int32.  Returns out [B, Hq, D].  Error bits: decode_errors(workspace)."""
+    if q.dim() == 4:
+        assert q.shape[1] == 1
+        q = q.squeeze(1)
+    _on_one_device(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, out, workspace)
+    b, hq, hd = q.shape
+    nb, bs, hk, hd2, t = _check_block_cache(k_cache, v_cache, k_scales, v_scales)
+    assert q.dtype == torch.bfloat16 and hd == hd2
+    assert b == 0 or (q.stride(2) == 1 and q.stride(1) == hd)
+    assert block_tables.dtype == torch.int32 and block_tables.stride(1) == 1 and block_tables.shape[0] >= b
+    assert context_lens.dtype == torch.int32 and context_lens.is_contiguous() and context_lens.numel() >= b
+    if out is None:
+        out = torch.empty(b, hq, hd, dtype=torch.bfloat16, device=q.device)
+    assert out.dtype == torch.bfloat16 and out.shape == (b, hq, hd) and out.stride(2) == 1 and out.stride(1) == hd
+    if b == 0:
+        return out
+    if workspace is None:
+        workspace = make_block_decode_workspace(b, hq, hk, q.device)
+    assert workspace.dtype == torch.uint8 and workspace.is_contiguous()
+    qrs, ors = (q.stride(0), out.stride(0)) if b > 1 else (hq * hd, hq * hd)
+    _launch(
+        "hl_paged_decode_fp8_blocks", q, q.data_ptr(), qrs, k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
+        block_tables.shape[1], context_lens.data_ptr(), b, hq, hk, hd, bs, t, nb, float(softmax_scale), out.data_ptr(),
+        ors, workspace.data_ptr(), workspace.numel())
+    return out
+
+
+# ------------------------------------------------------------------------ log probabilities
+def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_n: int = 0):
+    """Per row of logits [rows, V] (bf16 or fp32): the log probability of token_ids[row] (int64; -inf
+    outside the vocabulary), the entropy of the row's distribution and its top_n <= 32 most probable
+    tokens, lowest id first among equals (hl_token_logprobs).  Returns (logprobs [rows], entropies
+    [rows], top_tokens [rows, top_n] int64, top_logprobs [rows, top_n]), fp32."""
+    _on_one_device(logits, token_ids)
+    rows, vocab = logits.shape
+    assert logits.dtype in (torch.bfloat16, torch.float32) and (logits.stride(1) == 1 or vocab == 1)
+    assert token_ids.dtype == torch.int64 and token_ids.is_contiguous() and token_ids.shape == (rows,)
+    dev = logits.device
+    logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropies = torch.empty(rows, dtype=torch.float32, device=dev)
+    top_tokens = torch.empty(rows, top_n, dtype=torch.int64, device=dev)
+    top_logprobs = torch.empty(rows, top_n, dtype=torch.float32, device=dev)
+    _launch(
+        "hl_token_logprobs", logits, logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, logits.stride(0) if
+        rows > 1 else vocab, rows, vocab, token_ids.data_ptr(), int(top_n), logprobs.data_ptr(), entropies.data_ptr(),
+        top_tokens.data_ptr(), top_logprobs.data_ptr())
+    return logprobs, entropies, top_tokens, top_logprobs

@@ -401,6 +401,92 @@ int hl_sample_filtered(const void* logits, int64_t row_stride, int rows, int voc
                        const float* temperatures, const int32_t* top_ks, const float* top_ps,
                        uint64_t seed, void* step_state, int64_t* out_tokens, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Block tables and slot maps of a batch, built on the GPU from request lengths.
+ * Device form of BlockManager.allocate's page walk without the prefix cache
+ * (mini_vllm/engine/block_manager.py:58-80) and of prepare_prefill's metadata
+ * (mini_vllm/engine/model_runner.py:614-650), for callers whose lengths and free list are on the
+ * device.  Sequence b holds cached_lens[b] tokens in the first ceil(cached / block_size) entries of
+ * its block-table row (left as they are) and gets query_lens[b] more (negative lengths count as 0):
+ *   - the further pages it needs are the next ids of free_blocks, sequence after sequence; the rest
+ *     of its row becomes -1 (up to max_blocks);
+ *   - cu_seqlens_q / cu_seqlens_k [num_seqs + 1]: prefix sums of query and of cached + query;
+ *     context_lens [num_seqs] = cached + query;
+ *   - token i of the batch, i < max_tokens: positions[i] and slot_mapping[i] = page * block_size +
+ *     offset; -1 for a token without a page.  Entries behind the last token get position 0, slot -1.
+ * status [2]: pages taken from free_blocks, then HL_TABLES_* bits; where a bit is set the pages or
+ * tokens that do not fit are left out (-1) and everything else is as described.  num_seqs <= 4096;
+ * the totals, and every slot, must stay below 2^31 (a slot that does not gets -1).
+ * cached_lens may be NULL (all 0).
+ * ---------------------------------------------------------------------------------- */
+#define HL_TABLES_NO_PAGES 1         /* free_blocks is too short */
+#define HL_TABLES_TOO_NARROW 2       /* a sequence needs more than max_blocks pages */
+#define HL_TABLES_TOO_MANY_TOKENS 4  /* the query lengths add up to more than max_tokens */
+
+int hl_extend_block_tables(const int32_t* cached_lens, const int32_t* query_lens, int num_seqs,
+                           int32_t* block_tables, int64_t bt_stride, int max_blocks,
+                           const int32_t* free_blocks, int64_t num_free, int block_size, int64_t max_tokens,
+                           int32_t* cu_seqlens_q, int32_t* cu_seqlens_k, int32_t* context_lens,
+                           int64_t* positions, int32_t* slot_mapping, int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * 8-bit KV cache with a scale per block of tokens and head.  Caches [num_blocks, block_size, Hk, 128]
+ * e4m3 as above; k_scales / v_scales [num_blocks, block_size / scale_block, Hk] fp32; a value stands
+ * for e4m3 * scale of its group (scale_block consecutive slots of a page, one head).  scale_block is
+ * a multiple of 64 that divides block_size.  Unlike the per-head scales of hl_store_kv_fp8
+ * (mini_vllm/layers/attention.py:51-52,133 has none), these follow the data.
+ *
+ * hl_store_kv_fp8_blocks stores the new tokens of num_seqs sequences: rows cu_seqlens_q[b] ..
+ * cu_seqlens_q[b+1]-1 of key / value are tokens context_lens[b] - n .. context_lens[b]-1 of sequence
+ * b (cu_seqlens_q = NULL: one row per sequence), their pages the entries of its block-table row.
+ * Per group and head: scale := max(its scale if the group holds tokens from before this call, the
+ * smallest power of two s with max|x| / s <= 448 over the new rows, 2^-100); tokens from before are
+ * rescaled (round to nearest even) when it grows, new ones are e4m3(x / scale), saturating.
+ * Infinities and NaN do not set a scale; they are stored as +-448 and NaN.  Rows with no position
+ * >= 0, no table entry, or a page outside [0, num_blocks) are skipped, as are rows behind
+ * cu_seqlens_q[num_seqs].  A page that is written to belongs to one sequence.
+ * ---------------------------------------------------------------------------------- */
+int hl_store_kv_fp8_blocks(const void* key, const void* value, int64_t key_row_stride,
+                           int64_t value_row_stride, int64_t num_tokens, void* k_cache, void* v_cache,
+                           float* k_scales, float* v_scales, const int32_t* block_tables,
+                           int64_t bt_stride, int max_blocks_per_seq, const int32_t* context_lens,
+                           const int32_t* cu_seqlens_q, int num_seqs, int num_kv_heads, int head_dim,
+                           int block_size, int scale_block, int64_t num_blocks, void* stream);
+
+/* Decode attention over that cache: hl_paged_decode's arguments and result with the scales of the
+ * groups in place of per-head ones (mini_vllm/layers/attention.py:134-141).  Scales may be any
+ * finite fp32 values.  head_dim == 128, any Hk, Hq / Hk <= 16, batch <= 4096.  Tokens on a page
+ * outside [0, num_blocks) are left out and set bit 1 of the error word; contexts end at the table's
+ * width; rows with context_lens <= 0 give zeros.  The workspace must be zero-filled once before
+ * first use and is left ready for the next launch; launches that share it must not overlap.  Its
+ * first word holds the error bits (hl_paged_decode_read_errors). */
+int64_t hl_paged_decode_fp8_blocks_workspace_size(int batch, int num_q_heads, int num_kv_heads);
+
+int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, const void* k_cache,
+                               const void* v_cache, const float* k_scales, const float* v_scales,
+                               const int32_t* block_tables, int64_t bt_stride, int max_blocks_per_seq,
+                               const int32_t* context_lens, int batch, int num_q_heads,
+                               int num_kv_heads, int head_dim, int block_size, int scale_block,
+                               int64_t num_blocks, float softmax_scale, void* out,
+                               int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
+                               void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Log probabilities of given tokens with entropy and alternatives, for rows of logits (bf16, or
+ * fp32 with logits_fp32 = 1).  The reference's sampler returns token ids only
+ * (mini_vllm/layers/sampler.py:12-25).  Per row, with p = softmax(logits) in fp32:
+ *   logprobs[row] = ln p[token_ids[row]]  (-inf for an id outside [0, vocab));
+ *   entropies[row] = -sum p ln p;
+ *   top_tokens / top_logprobs [rows, top_n]: the top_n <= min(32, vocab) most probable tokens, most
+ *   probable first, the lowest id first among equals (top_n = 0: both may be NULL).
+ * A -inf logit is a masked token: probability 0.  A row with nothing else gives -inf, entropy 0 and
+ * the lowest ids; a NaN or +inf in a row makes its log probabilities and entropy NaN, NaN logits
+ * ranking last.
+ * ---------------------------------------------------------------------------------- */
+int hl_token_logprobs(const void* logits, int logits_fp32, int64_t row_stride, int64_t rows, int vocab,
+                      const int64_t* token_ids, int top_n, float* logprobs, float* entropies,
+                      int64_t* top_tokens, float* top_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
