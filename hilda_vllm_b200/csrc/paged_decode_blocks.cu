@@ -1,15 +1,47 @@
 // Paged decode attention (one query token per sequence) over the block-scaled 8-bit KV cache:
 //   out[b, hq] = sum_j p_j vs[g(j), h] Vq[j, h],  p = softmax_j(scale * ks[g(j), h] * q[b, hq] . Kq[j, h])
-// over the tokens j < context_lens[b] of sequence b, h = hq / (Hq / Hk), g(j) the group of
+// over the tokens j < context_lens[b] of sequence b, h = hq / G, G = Hq / Hk, g(j) the group of
 // scale_block tokens that j's slot lies in.  mini_vllm/layers/attention.py:134-141 calls an 8-bit
 // decode without scales.
+//
+// Bound: HBM, 256 B of K and V per token and head.  One warp walks 32-token tiles of one KV head
+// with an online softmax; K and V tiles arrive by cp.async in a ring of three 4 KiB slots of its own
+// (rows of 128 B, 16-byte chunks permuted so that every ld.shared.128 below is conflict-free), so
+// 8 KiB a warp are always in flight and no warp waits for another.
+//
+// Both products run on m16n8k16 f16 MMAs with the cache as the A operand, the G query heads being
+// the 8 (16 for G > 8) columns: every cache byte is converted once (e4m3 -> f16, exact) and used by
+// all G heads.  S^T = K Q^T: M = tokens; a lane's 32-bit word of a K row is its k-slice of one MMA, so
+// the dimensions are summed in a permuted order that Q's fragments share.  O^T = V^T P^T: M =
+// dimensions, a lane's pairs are two tokens' bytes of one dimension (byte permutes), P^T comes from
+// the S^T accumulators by an 8x8 transpose.  q is bf16 times an exact power of two per head, f16.
+// P is rounded to f16 (2^-12 relative to the tile's largest) against the tile's own maximum, each
+// tile's O^T is accumulated from zero and enters the fp32 running sum with exp2(m_tile - m) * vs, so
+// scales of any range cost no precision.  Maximum, sum and output are fp32.
+//
+// Work split: the tiles of all sequences in a row are cut into equal ranges, one per warp and head
+// (Hk neighbouring warps read the Hk heads of the same tokens, a contiguous piece of the cache).  A
+// sequence inside one range is written out directly; the parts of one cut across ranges go to the
+// workspace and the warp that finishes last merges them in range order (tickets; results do not
+// depend on the order of arrival).  More than kMergeFan parts are merged in two levels, so that the
+// ~300 parts of one long sequence are not read by a single warp.
 #include "kv_blocks.cuh"
+
+#include <atomic>
 
 namespace hl {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxBatch = 4096;
+constexpr int kWarps = 8;
+constexpr int kTile = 32;                           // tokens of one tile
+constexpr int kTileBytes = kTile * kBlockHeadDim;   // one ring slot
+constexpr int kSlots = 3;
+constexpr int kMaxCtas = 296;                       // two per SM of a B200
+constexpr int kMaxRanges = kMaxCtas * kWarps;       // (range, head) pairs at most
+constexpr int kMergeFan = 16;
+constexpr int kMaxDevices = 64;
 
 struct BlockDecodeParams {
   const __nv_bfloat16* q;
@@ -22,63 +54,568 @@ struct BlockDecodeParams {
   int64_t bt_stride;
   int max_blocks;
   const int32_t* context_lens;
-  int batch, num_q_heads, num_kv_heads;
+  int batch, group, num_kv_heads;
   int block_size, scale_block;
   int64_t num_blocks;
   float scale_log2;
   __nv_bfloat16* out;
   int64_t out_stride;
   int32_t* errors;
+  int32_t* tickets;      // [batch][Hk], all parts of a sequence
+  int32_t* sub_tickets;  // [2 * ranges][Hk], one group of kMergeFan parts
+  float2* part_ml;       // [2 * ranges][Hk][G]: (m, l)
+  float* part_o;         // [2 * ranges][Hk][G][128]
 };
 
-constexpr int kWarps = 8;
+// Workspace: error word | tickets | sub-tickets | (m, l) | o.
+struct WsLayout {
+  int64_t sub, ml, o, end;
+};
+__host__ __device__ inline WsLayout ws_layout(int batch, int num_q_heads, int num_kv_heads) {
+  const int64_t parts = 2 * int64_t(kMaxRanges / num_kv_heads);
+  WsLayout w;
+  w.sub = 256 + (int64_t(batch) * num_kv_heads * 4 + 255) / 256 * 256;
+  w.ml = w.sub + (parts * num_kv_heads * 4 + 255) / 256 * 256;
+  w.o = w.ml + (parts * num_q_heads * 8 + 255) / 256 * 256;
+  w.end = w.o + parts * num_q_heads * kBlockHeadDim * 4;
+  return w;
+}
 
-// One thread block per (query head, sequence); warp w takes tokens w, w + 8, ...; a lane holds four
-// of the 128 dimensions.
-__global__ void __launch_bounds__(32 * kWarps) decode_blocks_kernel(const BlockDecodeParams p) {
-  const int hq = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = hq / (p.num_q_heads / p.num_kv_heads);
-  const int64_t row_bytes = int64_t(p.num_kv_heads) * kBlockHeadDim;
-  const int64_t n = min(int64_t(p.context_lens[b]), int64_t(p.max_blocks) * p.block_size);
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  const uint2 qv = *reinterpret_cast<const uint2*>(p.q + b * p.q_stride + hq * kBlockHeadDim + 4 * lane);
-  q[0] = bf16lo(qv.x), q[1] = bf16hi(qv.x), q[2] = bf16lo(qv.y), q[3] = bf16hi(qv.y);
-  for (int64_t j = warp; j < n; j += kWarps) {
-    const int64_t page = p.block_tables[b * p.bt_stride + j / p.block_size];
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t e4m3_to_f16x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+// One warp's ring slot: the tile, then its group's scale and the number of tokens it holds.
+struct __align__(16) Slot {
+  uint8_t rows[kTileBytes];
+  float scale;
+  int32_t valid;
+  int32_t pad[2];
+};
+
+// Chunk permutation of a row: rows 2i, 2i + 1 (K: lanes 0-7 read two rows) and rows 0, 2, 4, 6 (V: four
+// rows, two chunks) fall into different banks.
+__device__ __forceinline__ int row_swizzle(int row) { return (row & 6) ^ ((row & 1) << 2); }
+
+// Walks the tiles [u, end) of the flattened list and issues their loads, K then V of each.
+struct Loader {
+  int u, end;      // next tile, end of the range
+  int b, b_end;    // its sequence, and that sequence's first tile index behind it
+  int n;           // tokens left in the sequence from this tile on
+  int page_at, off, group_off, group;  // table index, token offset in the page, in its group; group in the page
+  int64_t page;    // block id, or -1
+
+  __device__ __forceinline__ void read_page(const BlockDecodeParams& p) {
+    page = p.block_tables[b * p.bt_stride + page_at];
     if (page < 0 || page >= p.num_blocks) {
-      if (lane == 0) atomicOr(p.errors, 2);
-      continue;
+      if ((threadIdx.x & 31) == 0) atomicOr(p.errors, 2);
+      page = -1;
     }
-    const int64_t slot = page * p.block_size + j % p.block_size;
-    const int64_t at = slot * row_bytes + h * kBlockHeadDim + 4 * lane, sc = slot / p.scale_block * p.num_kv_heads + h;
-    const uint32_t kb = *reinterpret_cast<const uint32_t*>(p.k_cache + at);
-    const uint32_t vb = *reinterpret_cast<const uint32_t*>(p.v_cache + at);
-    const float2 k0 = e4m3x2_to_float2(kb & 0xffffu), k1 = e4m3x2_to_float2(kb >> 16);
-    const float2 v0 = e4m3x2_to_float2(vb & 0xffffu), v1 = e4m3x2_to_float2(vb >> 16);
-    float s = q[0] * k0.x + q[1] * k0.y + q[2] * k1.x + q[3] * k1.y;
-#pragma unroll
-    for (int t = 16; t >= 1; t >>= 1) s += __shfl_xor_sync(0xffffffffu, s, t);
-    s *= p.k_scales[sc] * p.scale_log2;
-    const float m2 = fmaxf(m, s), a = m == -INFINITY ? 0.f : exp2f(m - m2), e = s == -INFINITY ? 0.f : exp2f(s - m2);
-    const float ev = e * p.v_scales[sc];
-    l = l * a + e;
-    o[0] = o[0] * a + ev * v0.x, o[1] = o[1] * a + ev * v0.y, o[2] = o[2] * a + ev * v1.x, o[3] = o[3] * a + ev * v1.y;
-    m = m2;
   }
-  __shared__ float sm[kWarps], sl[kWarps], so[kWarps][kBlockHeadDim];
-  if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-  for (int t = 0; t < 4; ++t) so[warp][4 * lane + t] = o[t];
-  __syncthreads();
-  if (threadIdx.x >= kBlockHeadDim) return;
-  float mm = -INFINITY, ll = 0.f, oo = 0.f;
-  for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm[w]);
-  for (int w = 0; w < kWarps; ++w) {
-    const float a = sm[w] == -INFINITY ? 0.f : exp2f(sm[w] - mm);
-    ll += sl[w] * a;
-    oo += so[w][threadIdx.x] * a;
+  __device__ __forceinline__ void enter(const BlockDecodeParams& p, const int* prefix) {
+    const int first = u - prefix[b];  // tile of the sequence
+    const int ctx = min(p.context_lens[b], int(int64_t(p.max_blocks) * p.block_size));
+    const int tok = first * kTile;
+    n = ctx - tok;
+    b_end = prefix[b + 1];
+    page_at = tok / p.block_size;
+    off = tok - page_at * p.block_size;
+    group = off / p.scale_block;
+    group_off = off - group * p.scale_block;
+    read_page(p);
   }
-  p.out[b * p.out_stride + hq * kBlockHeadDim + threadIdx.x] = __float2bfloat16_rn(ll > 0.f || ll != ll ? oo / ll : 0.f);
+  __device__ __forceinline__ void load(const BlockDecodeParams& p, const uint8_t* cache, const float* scales, int h,
+                                       Slot* slot, int lane) const {
+    if (u < end) {
+      const int valid = page < 0 ? 0 : min(n, kTile);
+      const int64_t row_bytes = int64_t(p.num_kv_heads) * kBlockHeadDim;
+      const int r0 = lane >> 3, chunk = lane & 7;
+      const int64_t pg = page < 0 ? 0 : page;
+      const uint8_t* src = cache + (pg * p.block_size + off + r0) * row_bytes + h * kBlockHeadDim + chunk * 16;
+      const uint32_t dst = smem_u32(slot->rows) + r0 * kBlockHeadDim;
+      if (valid == kTile) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          cp_async16(dst + i * 4 * kBlockHeadDim + ((chunk ^ row_swizzle(r0 + 4 * i)) << 4), src + i * 4 * row_bytes, 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool in = r0 + 4 * i < valid;  // rows behind the context are zero, never read
+          cp_async16(dst + i * 4 * kBlockHeadDim + ((chunk ^ row_swizzle(r0 + 4 * i)) << 4),
+                     in ? src + i * 4 * row_bytes : cache, in ? 16 : 0);
+        }
+      }
+      if (lane == 0) {
+        slot->valid = valid;
+        if (valid > 0)
+          cp_async4(smem_u32(&slot->scale),
+                    scales + (pg * (p.block_size / p.scale_block) + group) * p.num_kv_heads + h);
+        else
+          slot->scale = 0.f;
+      }
+    }
+    cp_commit();
+  }
+  __device__ __forceinline__ void next(const BlockDecodeParams& p, const int* prefix) {
+    if (u >= end) return;
+    ++u;
+    if (u >= end) return;
+    if (u == b_end) {
+      do ++b; while (prefix[b + 1] == u);  // sequences without tokens have no tiles
+      enter(p, prefix);
+      return;
+    }
+    n -= kTile;
+    off += kTile;
+    group_off += kTile;
+    if (group_off == p.scale_block) group_off = 0, ++group;
+    if (off == p.block_size) {
+      off = 0, group = 0, ++page_at;
+      read_page(p);
+    }
+  }
+};
+
+// (m, l, o) of NP parts first, first + step, ... of one (sequence, head), merged in that order into
+// out (bf16, when final) or back into part `first`.
+__device__ void merge_parts(const BlockDecodeParams& p, int h, int first_slot, int first, int step, int count, int b,
+                            bool final, int lane) {
+  for (int g = 0; g < p.group; ++g) {
+    auto index = [&](int i) {  // part i of the list
+      const int r = first + i * step;
+      const int slot = r == first && first_slot ? 2 * r + 1 : 2 * r;
+      return (int64_t(slot) * p.num_kv_heads + h) * p.group + g;
+    };
+    float mm = -INFINITY;
+    for (int i = lane; i < count; i += 32) mm = fmaxf(mm, __ldcg(&p.part_ml[index(i)]).x);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < count; i0 += 32) {
+      float w = 0.f, wl = 0.f;
+      if (i0 + lane < count) {
+        const float2 ml = __ldcg(&p.part_ml[index(i0 + lane)]);
+        w = ex2(ml.x - ref);
+        wl = w * ml.y;
+      }
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) wl += __shfl_xor_sync(0xffffffffu, wl, o);
+      ll += wl;
+      const int k = min(32, count - i0);
+#pragma unroll 8
+      for (int i = 0; i < k; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + index(i0 + i) * kBlockHeadDim) + lane);
+        acc.x = fmaf(v.x, wi, acc.x);
+        acc.y = fmaf(v.y, wi, acc.y);
+        acc.z = fmaf(v.z, wi, acc.z);
+        acc.w = fmaf(v.w, wi, acc.w);
+      }
+    }
+    if (final) {
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
+      const __nv_bfloat162 hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(p.out + b * p.out_stride + (int64_t(h) * p.group + g) * kBlockHeadDim + 4 * lane) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    } else {
+      const int64_t at = index(0);
+      __syncwarp();
+      __stcg(reinterpret_cast<float4*>(p.part_o + at * kBlockHeadDim) + lane, acc);
+      if (lane == 0) __stcg(&p.part_ml[at], make_float2(mm, ll));
+    }
+  }
+}
+
+// True for the warp that takes the last of `count` tickets; it leaves the counter at zero.
+__device__ __forceinline__ bool last_ticket(int32_t* ticket, int count, int lane) {
+  __threadfence();
+  __syncwarp();
+  int last = 0;
+  if (lane == 0) {
+    last = atomicAdd(ticket, 1) == count - 1;
+    if (last) *ticket = 0;
+  }
+  last = __shfl_sync(0xffffffffu, last, 0);
+  if (last) __threadfence();
+  return last;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_kernel(const BlockDecodeParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Slot* ring = reinterpret_cast<Slot*>(smem) + warp * kSlots;
+  int* prefix = reinterpret_cast<int*>(smem + sizeof(Slot) * kSlots * kWarps);  // [batch + 1] first tiles
+  __shared__ int warp_sum[kWarps];
+
+  // Tiles of each sequence and their prefix sums.
+  {
+    const int per = (p.batch + 32 * kWarps - 1) / (32 * kWarps);
+    const int width = int(int64_t(p.max_blocks) * p.block_size);
+    const int b0 = threadIdx.x * per;
+    int sum = 0;
+    for (int i = 0; i < per; ++i) {
+      const int b = b0 + i;
+      if (b < p.batch) sum += (max(min(p.context_lens[b], width), 0) + kTile - 1) / kTile;
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int before = incl - sum;
+    for (int w = 0; w < warp; ++w) before += warp_sum[w];
+    for (int i = 0; i < per; ++i) {
+      const int b = b0 + i;
+      if (b < p.batch) {
+        prefix[b] = before;
+        before += (max(min(p.context_lens[b], width), 0) + kTile - 1) / kTile;
+        if (b == p.batch - 1) prefix[p.batch] = before;
+      }
+    }
+    __syncthreads();
+  }
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (prefix[b] != prefix[b + 1]) continue;
+    uint4* o = reinterpret_cast<uint4*>(p.out + b * p.out_stride);
+    for (int i = threadIdx.x; i < p.group * p.num_kv_heads * (kBlockHeadDim / 8); i += 32 * kWarps) o[i] = make_uint4(0, 0, 0, 0);
+  }
+
+  const int total = prefix[p.batch];
+  const int gid = blockIdx.x * kWarps + warp;
+  const int h = gid % p.num_kv_heads, range = gid / p.num_kv_heads;
+  const int ranges = min(int(gridDim.x) * kWarps / p.num_kv_heads, total);
+  if (range >= ranges) return;
+  auto range_begin = [&](int r) { return int(int64_t(r) * total / ranges); };
+  auto range_of = [&](int u) {  // the range that tile u lies in
+    return int((int64_t(u) * ranges + ranges - 1) / total);
+  };
+  Loader ld;
+  ld.u = range_begin(range);
+  ld.end = range_begin(range + 1);
+  int lo = 0, hi = p.batch - 1;  // last sequence that begins at or before the tile and has tiles
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= ld.u) lo = mid; else hi = mid - 1;
+  }
+  ld.b = lo;
+  ld.enter(p, prefix);
+  int b = ld.b;
+  int u = ld.u;
+  const int end = ld.end;
+  ld.load(p, p.k_cache, p.k_scales, h, ring + 0, lane);
+  ld.load(p, p.v_cache, p.v_scales, h, ring + 1, lane);
+  ld.next(p, prefix);
+  ld.load(p, p.k_cache, p.k_scales, h, ring + 2, lane);
+
+  const int c = lane & 3, rr = lane >> 2;
+  int slot = 0;
+  while (u < end) {
+    // ---- one sequence: its query heads as B fragments
+    uint32_t qf[NT][8][2];
+    float qs[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int g = t * 8 + rr;
+      uint32_t w[2][8];
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
+        if (g < p.group) {
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.q_stride + (int64_t(h) * p.group + g) * kBlockHeadDim +
+                                                            16 * (c + 4 * i));
+          v0 = __ldg(src);
+          v1 = __ldg(src + 1);
+        }
+        w[i][0] = v0.x, w[i][1] = v0.y, w[i][2] = v0.z, w[i][3] = v0.w;
+        w[i][4] = v1.x, w[i][5] = v1.y, w[i][6] = v1.z, w[i][7] = v1.w;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fmaxf(fabsf(bf16lo(w[i][k])), fabsf(bf16hi(w[i][k]))));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // The power of two that brings the largest |q| of the head into [2^10, 2^11).
+      float up = 1.f, down = 1.f;
+      if (amax > 0.f && amax < INFINITY) {
+        const int e = max(min(264 - int(__float_as_uint(amax) >> 23), 253), 1);
+        up = __uint_as_float(uint32_t(e) << 23);
+        down = __uint_as_float(uint32_t(254 - e) << 23);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            qf[t][4 * i + k][x] = pack_half2(bf16lo(w[i][2 * k + x]) * up, bf16hi(w[i][2 * k + x]) * up);
+      qs[t][0] = __shfl_sync(0xffffffffu, down, 8 * c) * p.scale_log2;
+      qs[t][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4) * p.scale_log2;
+    }
+    float m[NT][2], l[NT][2], o[NT][8][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) m[t][x] = -INFINITY, l[t][x] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[t][j][x] = 0.f;
+    }
+    const int seq_end = prefix[b + 1], seq_begin = prefix[b];
+    const bool begins = u == seq_begin;
+    const int stop = min(end, seq_end);
+    for (; u < stop; ++u) {
+      // ---- S^T = K Q^T
+      cp_wait<2>();
+      __syncwarp();
+      float s[2][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[mt][t][x] = 0.f;
+      const uint32_t kbase = smem_u32(ring[slot].rows) + rr * kBlockHeadDim;
+      const int ksw = row_swizzle(rr);
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t at = kbase + mt * 16 * kBlockHeadDim + (((c + 4 * i) ^ ksw) << 4);
+          const uint4 ka = lds128(at), kb = lds128(at + 8 * kBlockHeadDim);
+          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t a0 = e4m3_to_f16x2(uint16_t(wa[w])), a2 = e4m3_to_f16x2(uint16_t(wa[w] >> 16));
+            const uint32_t a1 = e4m3_to_f16x2(uint16_t(wb[w])), a3 = e4m3_to_f16x2(uint16_t(wb[w] >> 16));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma_f16(s[mt][t], a0, a1, a2, a3, qf[t][4 * i + w][0], qf[t][4 * i + w][1]);
+          }
+        }
+      }
+      const float ks = ring[slot].scale;
+      const int valid = ring[slot].valid;
+      __syncwarp();
+      ld.load(p, p.v_cache, p.v_scales, h, ring + slot, lane);  // V of the next tile
+      ld.next(p, prefix);
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
+
+      // ---- softmax of the tile against its own maximum
+      uint32_t pf[NT][2][2];
+      float alpha[NT][2], beta[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float f = ks * qs[t][x];
+          float mx = -INFINITY;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float& v = s[mt][t][2 * y + x];
+              v = mt * 16 + y * 8 + rr < valid ? v * f : -INFINITY;
+              mx = fmaxf(mx, v);
+            }
+#pragma unroll
+          for (int k = 4; k <= 16; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+          const float m2 = fmaxf(m[t][x], mx);
+          const float ref = mx == -INFINITY ? 0.f : mx, ref2 = m2 == -INFINITY ? 0.f : m2;
+          alpha[t][x] = ex2(m[t][x] - ref2);
+          beta[t][x] = ex2(mx - ref2);
+          float sum = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float& v = s[mt][t][2 * y + x];
+              v = ex2(v - ref);
+              sum += v;
+            }
+          // A tile without a finite score: its exponentials are 0, or NaN if a score is.
+          l[t][x] = fmaf(l[t][x], alpha[t][x], mx == -INFINITY ? sum : sum * beta[t][x]);
+          m[t][x] = m2;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) pf[t][mt][y] = transpose8x8(pack_half2(s[mt][t][2 * y], s[mt][t][2 * y + 1]));
+      }
+
+      // ---- O^T += V^T P^T
+      cp_wait<2>();
+      __syncwarp();
+      const uint32_t vbase = smem_u32(ring[slot].rows);
+      uint4 v[2][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = mt * 16 + 2 * c + (k & 1) + (k >> 1) * 8;
+          v[mt][k] = lds128(vbase + row * kBlockHeadDim + ((rr ^ row_swizzle(row)) << 4));
+        }
+      const float vs = ring[slot].scale;
+      __syncwarp();
+      ld.load(p, p.k_cache, p.k_scales, h, ring + slot, lane);  // K of the tile after the next
+      slot = slot == kSlots - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) beta[t][0] *= vs, beta[t][1] *= vs;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t sel = half ? 0x7362u : 0x5140u;
+          float acc[NT][4];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[t][x] = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            auto word = [&](int k) { return w == 0 ? v[mt][k].x : w == 1 ? v[mt][k].y : w == 2 ? v[mt][k].z : v[mt][k].w; };
+            const uint32_t e = __byte_perm(word(0), word(1), sel), f = __byte_perm(word(2), word(3), sel);
+            const uint32_t a0 = e4m3_to_f16x2(uint16_t(e)), a1 = e4m3_to_f16x2(uint16_t(e >> 16));
+            const uint32_t a2 = e4m3_to_f16x2(uint16_t(f)), a3 = e4m3_to_f16x2(uint16_t(f >> 16));
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma_f16(acc[t], a0, a1, a2, a3, pf[t][mt][0], pf[t][mt][1]);
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              o[t][2 * w + half][x] = fmaf(acc[t][x], beta[t][x & 1], o[t][2 * w + half][x] * alpha[t][x & 1]);
+        }
+      }
+    }
+
+    // ---- the sequence (or its part in this range) is done
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int k = 4; k <= 16; k <<= 1) l[t][x] += __shfl_xor_sync(0xffffffffu, l[t][x], k);
+    if (begins && stop == seq_end) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int g = t * 8 + 2 * c + x;
+          if (g >= p.group) continue;
+          const float inv = l[t][x] == 0.f ? 0.f : 1.f / l[t][x];
+          uint32_t w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const __nv_bfloat162 h2 = __floats2bfloat162_rn(o[t][j][x] * inv, o[t][j][2 + x] * inv);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h2);
+          }
+          uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.out_stride + (int64_t(h) * p.group + g) * kBlockHeadDim + 16 * rr);
+          dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
+    } else {
+      const int64_t part = (int64_t(2 * range + (begins ? 1 : 0)) * p.num_kv_heads + h) * p.group;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int g = t * 8 + 2 * c + x;
+          if (g >= p.group) continue;
+          float4* dst = reinterpret_cast<float4*>(p.part_o + (part + g) * kBlockHeadDim + 16 * rr);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            __stcg(dst + j, make_float4(o[t][2 * j][x], o[t][2 * j][2 + x], o[t][2 * j + 1][x], o[t][2 * j + 1][2 + x]));
+          if (rr == 0) __stcg(&p.part_ml[part + g], make_float2(m[t][x], l[t][x]));
+        }
+      const int first = range_of(seq_begin), last = range_of(seq_end - 1), parts = last - first + 1;
+      int32_t* ticket = p.tickets + int64_t(b) * p.num_kv_heads + h;
+      if (parts <= kMergeFan) {
+        if (last_ticket(ticket, parts, lane)) merge_parts(p, h, 1, first, 1, parts, b, true, lane);
+      } else {
+        const int sub = (range - first) / kMergeFan, subs = (parts + kMergeFan - 1) / kMergeFan;
+        const int head = first + sub * kMergeFan, count = min(kMergeFan, last - head + 1);
+        const int head_slot = 2 * head + (sub == 0 ? 1 : 0);
+        if (last_ticket(p.sub_tickets + int64_t(head_slot) * p.num_kv_heads + h, count, lane)) {
+          merge_parts(p, h, sub == 0, head, 1, count, b, false, lane);
+          if (last_ticket(ticket, subs, lane)) merge_parts(p, h, 1, first, kMergeFan, subs, b, true, lane);
+        }
+      }
+    }
+    do ++b; while (u < end && prefix[b + 1] == u);
+  }
+  cp_wait<0>();
+}
+
+template <int NT>
+int launch_decode_blocks(const BlockDecodeParams& p, cudaStream_t s) {
+  constexpr int kPerSm = NT == 1 ? 2 : 1;
+  constexpr int kSlotBytes = int(sizeof(Slot)) * kSlots * kWarps;
+  static std::atomic<int> sms[kMaxDevices];  // 0: this kernel is not set up on the device yet
+  int dev = -1;
+  cudaError_t e = cudaGetDevice(&dev);
+  int n = e == cudaSuccess && dev < kMaxDevices ? sms[dev].load(std::memory_order_relaxed) : 0;
+  if (e == cudaSuccess && n == 0) {
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(decode_blocks_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kSlotBytes + 4 * (kMaxBatch + 1));
+    if (e == cudaSuccess && dev < kMaxDevices) sms[dev].store(n, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) {
+    set_error("hl_paged_decode_fp8_blocks: %s", cudaGetErrorString(e));
+    return HL_ERR_CUDA;
+  }
+  int ctas = n * kPerSm < kMaxCtas ? n * kPerSm : kMaxCtas;
+  if (ctas * kWarps < p.num_kv_heads) ctas = (p.num_kv_heads + kWarps - 1) / kWarps;
+  decode_blocks_kernel<NT><<<ctas, 32 * kWarps, kSlotBytes + 4 * (p.batch + 1), s>>>(p);
+  HL_CHECK_LAUNCH("hl_paged_decode_fp8_blocks");
+  return HL_OK;
 }
 
 }  // namespace
@@ -88,7 +625,8 @@ using namespace hl;
 
 extern "C" int64_t hl_paged_decode_fp8_blocks_workspace_size(int batch, int num_q_heads, int num_kv_heads) {
   if (batch <= 0 || batch > kMaxBatch || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return -1;
-  return 256;
+  if (num_kv_heads > kMaxRanges) return -1;
+  return ws_layout(batch, num_q_heads, num_kv_heads).end;
 }
 
 extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, const void* k_cache,
@@ -112,8 +650,10 @@ extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, c
                "hl_paged_decode_fp8_blocks: scale_block must be a multiple of 64 that divides block_size");
   HL_CHECK_ARG(max_blocks_per_seq > 0 && bt_stride >= max_blocks_per_seq && num_blocks > 0,
                "hl_paged_decode_fp8_blocks: bad block table or pool shape");
-  HL_CHECK_ARG(int64_t(max_blocks_per_seq) * block_size <= 0x7fffffff,
-               "hl_paged_decode_fp8_blocks: a block table row spans 2^31 tokens or more");
+  HL_CHECK_ARG(int64_t(max_blocks_per_seq) * block_size <= 0x7fffffff &&
+                   int64_t(batch) * max_blocks_per_seq * (block_size / kTile) <= 0x7fffffff,
+               "hl_paged_decode_fp8_blocks: the block tables span 2^31 tokens a row or 2^36 in all");
+  HL_CHECK_ARG(num_kv_heads <= kMaxRanges, "hl_paged_decode_fp8_blocks: more than %d KV heads", kMaxRanges);
   HL_CHECK_ARG(aligned16(q) && q_row_stride % 8 == 0 && q_row_stride >= int64_t(num_q_heads) * head_dim &&
                    aligned16(out) && out_row_stride % 8 == 0 && out_row_stride >= int64_t(num_q_heads) * head_dim &&
                    aligned16(k_cache) && aligned16(v_cache),
@@ -136,7 +676,6 @@ extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, c
   p.max_blocks = max_blocks_per_seq;
   p.context_lens = context_lens;
   p.batch = batch;
-  p.num_q_heads = num_q_heads;
   p.num_kv_heads = num_kv_heads;
   p.block_size = block_size;
   p.scale_block = scale_block;
@@ -144,9 +683,14 @@ extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, c
   p.scale_log2 = softmax_scale * kLog2e;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.out_stride = out_row_stride;
-  p.errors = static_cast<int32_t*>(workspace);
-  const dim3 grid(num_q_heads, batch);
-  decode_blocks_kernel<<<grid, 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  HL_CHECK_LAUNCH("hl_paged_decode_fp8_blocks");
-  return HL_OK;
+  p.group = num_q_heads / num_kv_heads;
+  const WsLayout w = ws_layout(batch, num_q_heads, num_kv_heads);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.errors = reinterpret_cast<int32_t*>(ws);
+  p.tickets = reinterpret_cast<int32_t*>(ws + 256);
+  p.sub_tickets = reinterpret_cast<int32_t*>(ws + w.sub);
+  p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
+  p.part_o = reinterpret_cast<float*>(ws + w.o);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return p.group <= 8 ? launch_decode_blocks<1>(p, s) : launch_decode_blocks<2>(p, s);
 }
