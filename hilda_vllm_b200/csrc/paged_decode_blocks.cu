@@ -5,19 +5,21 @@
 // decode without scales.
 //
 // Bound: HBM, 256 B of K and V per token and head.  One warp walks 32-token tiles of one KV head
-// with an online softmax; K and V tiles arrive by cp.async in a ring of three 4 KiB slots of its own
-// (rows of 128 B, 16-byte chunks permuted so that every ld.shared.128 below is conflict-free), so
-// 8 KiB a warp are always in flight and no warp waits for another.
+// with an online softmax; its K and V tiles arrive by TMA (128-byte swizzle) in a ring of three
+// 4 KiB slots of its own, issued by a ninth warp whose lane w serves warp w, so page lookups and
+// copies run ahead of the arithmetic and no consumer waits for another.
 //
 // Both products run on m16n8k16 f16 MMAs with the cache as the A operand, the G query heads being
 // the 8 (16 for G > 8) columns: every cache byte is converted once (e4m3 -> f16, exact) and used by
 // all G heads.  S^T = K Q^T: M = tokens; a lane's 32-bit word of a K row is its k-slice of one MMA, so
 // the dimensions are summed in a permuted order that Q's fragments share.  O^T = V^T P^T: M =
 // dimensions, a lane's pairs are two tokens' bytes of one dimension (byte permutes), P^T comes from
-// the S^T accumulators by an 8x8 transpose.  q is bf16 times an exact power of two per head, f16.
-// P is rounded to f16 (2^-12 relative to the tile's largest) against the tile's own maximum, each
-// tile's O^T is accumulated from zero and enters the fp32 running sum with exp2(m_tile - m) * vs, so
-// scales of any range cost no precision.  Maximum, sum and output are fp32.
+// the S^T accumulators by an 8x8 transpose.  The MMA row r of a block of 8 is token tile_row(r), an
+// order in which every 16-byte shared load of K and of V is free of bank conflicts.
+// q is bf16 times an exact power of two per head, f16.  With lv = log2 vs of the tile, the weights
+// enter the second product as f16(2^(s + lv - M)), M the running maximum of s + lv, and the sum as
+// fp32 2^(s - m): scales of any range cost no precision, and the f16 rounding (2^-12) is relative to
+// the largest weighted value.  Maxima, sums and outputs are fp32; O is rescaled only when M grows.
 //
 // Work split: the tiles of all sequences in a row are cut into equal ranges, one per warp and head
 // (Hk neighbouring warps read the Hk heads of the same tokens, a contiguous piece of the cache).  A
@@ -26,6 +28,8 @@
 // depend on the order of arrival).  More than kMergeFan parts are merged in two levels, so that the
 // ~300 parts of one long sequence are not read by a single warp.
 #include "kv_blocks.cuh"
+
+#include <cuda.h>
 
 #include <atomic>
 
@@ -44,10 +48,9 @@ constexpr int kMergeFan = 16;
 constexpr int kMaxDevices = 64;
 
 struct BlockDecodeParams {
+  CUtensorMap k_map, v_map;  // [num_blocks * block_size rows][Hk * 128 B], boxes of 32 rows x 128 B
   const __nv_bfloat16* q;
   int64_t q_stride;
-  const uint8_t* k_cache;
-  const uint8_t* v_cache;
   const float* k_scales;
   const float* v_scales;
   const int32_t* block_tables;
@@ -93,69 +96,77 @@ __device__ __forceinline__ uint32_t e4m3_to_f16x2(uint16_t v) {
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done;
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
+// Copies one float and arrives on the barrier once it has landed.
+__device__ __forceinline__ void copy_float_arrive(float* dst, const float* src, uint64_t* bar) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// One warp's ring slot: the tile, then its group's scale and the number of tokens it holds.
-struct __align__(16) Slot {
-  uint8_t rows[kTileBytes];
-  float scale;
-  int32_t valid;
-  int32_t pad[2];
+// Token of MMA row r (mod 8).  K: lanes 0-7 of a shared load read rows 2i, 2i + 1, whose tokens
+// differ in bit 2; V: rows 0, 2, 4, 6 (or 1, 3, 5, 7) of two chunks, tokens that differ in bits 1-2.
+// The 128-byte swizzle XORs the 16-byte chunk with the token's low three bits: no conflicts.
+__device__ __forceinline__ int tile_row(int r) { return r ^ ((r & 1) << 2); }
+
+struct Shared {
+  uint8_t rows[kWarps][kSlots][kTileBytes];  // 1024-byte aligned slots
+  uint64_t full[kWarps][kSlots], empty[kWarps][kSlots];
+  float scale[kWarps][kSlots];
+  int32_t valid[kWarps][kSlots];  // tokens the tile holds; 0: its page is outside the pool
+  int32_t warp_sum[kWarps + 1];
+  int32_t pad;
+  int32_t prefix[];  // [batch + 1] first tile of each sequence
 };
 
-// Chunk permutation of a row: rows 2i, 2i + 1 (K: lanes 0-7 read two rows) and rows 0, 2, 4, 6 (V: four
-// rows, two chunks) fall into different banks.
-__device__ __forceinline__ int row_swizzle(int row) { return (row & 6) ^ ((row & 1) << 2); }
-
-// Walks the tiles [u, end) of the flattened list and issues their loads, K then V of each.
+// The producer lane of one consumer warp: walks the tiles [u, end) and copies K, then V of each into
+// the next ring slot that is empty.
 struct Loader {
   int u, end;      // next tile, end of the range
   int b, b_end;    // its sequence, and that sequence's first tile index behind it
   int n;           // tokens left in the sequence from this tile on
   int page_at, off, group_off, group;  // table index, token offset in the page, in its group; group in the page
-  int64_t page;    // block id, or -1
+  int page;        // block id, or -1
 
   __device__ __forceinline__ void read_page(const BlockDecodeParams& p) {
     page = p.block_tables[b * p.bt_stride + page_at];
     if (page < 0 || page >= p.num_blocks) {
-      if ((threadIdx.x & 31) == 0) atomicOr(p.errors, 2);
+      atomicOr(p.errors, 2);
       page = -1;
     }
   }
   __device__ __forceinline__ void enter(const BlockDecodeParams& p, const int* prefix) {
-    const int first = u - prefix[b];  // tile of the sequence
-    const int ctx = min(p.context_lens[b], int(int64_t(p.max_blocks) * p.block_size));
-    const int tok = first * kTile;
-    n = ctx - tok;
+    const int tok = (u - prefix[b]) * kTile;
+    n = min(p.context_lens[b], p.max_blocks * p.block_size) - tok;
     b_end = prefix[b + 1];
     page_at = tok / p.block_size;
     off = tok - page_at * p.block_size;
@@ -163,42 +174,25 @@ struct Loader {
     group_off = off - group * p.scale_block;
     read_page(p);
   }
-  __device__ __forceinline__ void load(const BlockDecodeParams& p, const uint8_t* cache, const float* scales, int h,
-                                       Slot* slot, int lane) const {
-    if (u < end) {
-      const int valid = page < 0 ? 0 : min(n, kTile);
-      const int64_t row_bytes = int64_t(p.num_kv_heads) * kBlockHeadDim;
-      const int r0 = lane >> 3, chunk = lane & 7;
-      const int64_t pg = page < 0 ? 0 : page;
-      const uint8_t* src = cache + (pg * p.block_size + off + r0) * row_bytes + h * kBlockHeadDim + chunk * 16;
-      const uint32_t dst = smem_u32(slot->rows) + r0 * kBlockHeadDim;
-      if (valid == kTile) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          cp_async16(dst + i * 4 * kBlockHeadDim + ((chunk ^ row_swizzle(r0 + 4 * i)) << 4), src + i * 4 * row_bytes, 16);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const bool in = r0 + 4 * i < valid;  // rows behind the context are zero, never read
-          cp_async16(dst + i * 4 * kBlockHeadDim + ((chunk ^ row_swizzle(r0 + 4 * i)) << 4),
-                     in ? src + i * 4 * row_bytes : cache, in ? 16 : 0);
-        }
-      }
-      if (lane == 0) {
-        slot->valid = valid;
-        if (valid > 0)
-          cp_async4(smem_u32(&slot->scale),
-                    scales + (pg * (p.block_size / p.scale_block) + group) * p.num_kv_heads + h);
-        else
-          slot->scale = 0.f;
-      }
+  __device__ __forceinline__ void load(const BlockDecodeParams& p, Shared& sh, int w, int slot, int h, bool v) const {
+    uint64_t* full = &sh.full[w][slot];
+    if (page < 0) {
+      sh.valid[w][slot] = 0;
+      sh.scale[w][slot] = 0.f;
+      mbar_arrive(full);
+      mbar_arrive(full);
+      return;
     }
-    cp_commit();
+    sh.valid[w][slot] = min(n, kTile);
+    mbar_arrive_expect_tx(full, kTileBytes);
+    tma_2d(sh.rows[w][slot], v ? &p.v_map : &p.k_map, h * kBlockHeadDim, page * p.block_size + off, full);
+    copy_float_arrive(&sh.scale[w][slot],
+                      (v ? p.v_scales : p.k_scales) +
+                          (int64_t(page) * (p.block_size / p.scale_block) + group) * p.num_kv_heads + h,
+                      full);
   }
   __device__ __forceinline__ void next(const BlockDecodeParams& p, const int* prefix) {
-    if (u >= end) return;
-    ++u;
-    if (u >= end) return;
+    if (++u >= end) return;
     if (u == b_end) {
       do ++b; while (prefix[b + 1] == u);  // sequences without tokens have no tiles
       enter(p, prefix);
@@ -215,7 +209,7 @@ struct Loader {
   }
 };
 
-// (m, l, o) of NP parts first, first + step, ... of one (sequence, head), merged in that order into
+// (m, l, o) of `count` parts first, first + step, ... of one (sequence, head), merged in that order into
 // out (bf16, when final) or back into part `first`.
 __device__ void merge_parts(const BlockDecodeParams& p, int h, int first_slot, int first, int step, int count, int b,
                             bool final, int lane) {
@@ -268,6 +262,9 @@ __device__ void merge_parts(const BlockDecodeParams& p, int h, int first_slot, i
   }
 }
 
+// 2^(mv - m), the factor from units of 2^mv to units of 2^m; 0 where nothing was summed.
+__device__ __forceinline__ float unit(float mv, float m) { return mv == -INFINITY ? 0.f : exp2f(mv - m); }
+
 // True for the warp that takes the last of `count` tickets; it leaves the counter at zero.
 __device__ __forceinline__ bool last_ticket(int32_t* ticket, int count, int lane) {
   __threadfence();
@@ -283,78 +280,116 @@ __device__ __forceinline__ bool last_ticket(int32_t* ticket, int count, int lane
 }
 
 template <int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_kernel(const BlockDecodeParams p) {
-  extern __shared__ __align__(16) uint8_t smem[];
+__global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
+    decode_blocks_kernel(const __grid_constant__ BlockDecodeParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem);
+  int* prefix = sh.prefix;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Slot* ring = reinterpret_cast<Slot*>(smem) + warp * kSlots;
-  int* prefix = reinterpret_cast<int*>(smem + sizeof(Slot) * kSlots * kWarps);  // [batch + 1] first tiles
-  __shared__ int warp_sum[kWarps];
-
+  if (threadIdx.x < kWarps * kSlots) {
+    mbar_init(&sh.full[0][0] + threadIdx.x, 2);   // the tile's bytes and the scale
+    mbar_init(&sh.empty[0][0] + threadIdx.x, 1);
+    fence_mbar_init();
+  }
   // Tiles of each sequence and their prefix sums.
   {
-    const int per = (p.batch + 32 * kWarps - 1) / (32 * kWarps);
-    const int width = int(int64_t(p.max_blocks) * p.block_size);
+    constexpr int kThreads = 32 * (kWarps + 1);
+    const int per = (p.batch + kThreads - 1) / kThreads, width = p.max_blocks * p.block_size;
     const int b0 = threadIdx.x * per;
     int sum = 0;
-    for (int i = 0; i < per; ++i) {
-      const int b = b0 + i;
-      if (b < p.batch) sum += (max(min(p.context_lens[b], width), 0) + kTile - 1) / kTile;
-    }
+    for (int b = b0; b < min(b0 + per, p.batch); ++b) sum += (max(min(p.context_lens[b], width), 0) + kTile - 1) / kTile;
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    if (lane == 31) warp_sum[warp] = incl;
+    if (lane == 31) sh.warp_sum[warp] = incl;
     __syncthreads();
     int before = incl - sum;
-    for (int w = 0; w < warp; ++w) before += warp_sum[w];
-    for (int i = 0; i < per; ++i) {
-      const int b = b0 + i;
-      if (b < p.batch) {
-        prefix[b] = before;
-        before += (max(min(p.context_lens[b], width), 0) + kTile - 1) / kTile;
-        if (b == p.batch - 1) prefix[p.batch] = before;
-      }
+    for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
+    for (int b = b0; b < min(b0 + per, p.batch); ++b) {
+      prefix[b] = before;
+      before += (max(min(p.context_lens[b], width), 0) + kTile - 1) / kTile;
+      if (b == p.batch - 1) prefix[p.batch] = before;
     }
     __syncthreads();
   }
+  const int total = prefix[p.batch];
+  const int ranges = min(int(gridDim.x) * kWarps / p.num_kv_heads, total);
+  auto range_begin = [&](int r) { return int(int64_t(r) * total / ranges); };
+  auto range_of = [&](int u) { return int((int64_t(u) * ranges + ranges - 1) / total); };  // that tile u lies in
+  auto sequence_of = [&](int u) {  // the last sequence that begins at or before u: it has tiles
+    int lo = 0, hi = p.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  };
+
+  if (warp == kWarps) {
+    // ---- producer: lane w loads for warp w
+    const int gid = blockIdx.x * kWarps + lane;
+    const int h = gid % p.num_kv_heads, range = gid / p.num_kv_heads;
+    Loader ld;
+    ld.u = ld.end = 0;
+    if (lane < kWarps && range < ranges) {
+      ld.u = range_begin(range);
+      ld.end = range_begin(range + 1);
+      ld.b = sequence_of(ld.u);
+      ld.enter(p, prefix);
+    }
+    int slot = 0, round = 0, idle = 0;
+    bool v = false;
+    while (__any_sync(0xffffffffu, ld.u < ld.end)) {
+      if (ld.u < ld.end) {
+        if (mbar_test(&sh.empty[lane][slot], (round & 1) ^ 1)) {
+          ld.load(p, sh, lane, slot, h, v);
+          if (v) ld.next(p, prefix);
+          v = !v;
+          if (++slot == kSlots) slot = 0, ++round;
+          idle = 0;
+        } else {
+          if (++idle > int(kMaxWaitPolls)) {  // the consumer gave up
+            atomicOr(p.errors, 1);
+            ld.end = ld.u;
+          }
+          __nanosleep(40);
+        }
+      }
+      __syncwarp();
+    }
+    // Copies in flight that nobody will wait for (none unless a wait gave up).
+    if (idle) {
+      for (int i = 0; i < kSlots; ++i) {
+        const int at = slot - 1 - i, s = at < 0 ? at + kSlots : at, r = at < 0 ? round - 1 : round;
+        if (r >= 0) mbar_wait(&sh.full[lane][s], r & 1);
+      }
+    }
+    return;
+  }
+
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
     if (prefix[b] != prefix[b + 1]) continue;
     uint4* o = reinterpret_cast<uint4*>(p.out + b * p.out_stride);
     for (int i = threadIdx.x; i < p.group * p.num_kv_heads * (kBlockHeadDim / 8); i += 32 * kWarps) o[i] = make_uint4(0, 0, 0, 0);
   }
-
-  const int total = prefix[p.batch];
   const int gid = blockIdx.x * kWarps + warp;
   const int h = gid % p.num_kv_heads, range = gid / p.num_kv_heads;
-  const int ranges = min(int(gridDim.x) * kWarps / p.num_kv_heads, total);
   if (range >= ranges) return;
-  auto range_begin = [&](int r) { return int(int64_t(r) * total / ranges); };
-  auto range_of = [&](int u) {  // the range that tile u lies in
-    return int((int64_t(u) * ranges + ranges - 1) / total);
-  };
-  Loader ld;
-  ld.u = range_begin(range);
-  ld.end = range_begin(range + 1);
-  int lo = 0, hi = p.batch - 1;  // last sequence that begins at or before the tile and has tiles
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (prefix[mid] <= ld.u) lo = mid; else hi = mid - 1;
-  }
-  ld.b = lo;
-  ld.enter(p, prefix);
-  int b = ld.b;
-  int u = ld.u;
-  const int end = ld.end;
-  ld.load(p, p.k_cache, p.k_scales, h, ring + 0, lane);
-  ld.load(p, p.v_cache, p.v_scales, h, ring + 1, lane);
-  ld.next(p, prefix);
-  ld.load(p, p.k_cache, p.k_scales, h, ring + 2, lane);
+  int u = range_begin(range);
+  const int end = range_begin(range + 1);
+  int b = sequence_of(u);
 
   const int c = lane & 3, rr = lane >> 2;
   int slot = 0;
+  uint32_t parity = 0;
+  auto advance = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.empty[warp][slot]);
+    if (++slot == kSlots) slot = 0, parity ^= 1;
+  };
   while (u < end) {
     // ---- one sequence: its query heads as B fragments
     uint32_t qf[NT][8][2];
@@ -397,11 +432,12 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_ke
       qs[t][0] = __shfl_sync(0xffffffffu, down, 8 * c) * p.scale_log2;
       qs[t][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4) * p.scale_log2;
     }
-    float m[NT][2], l[NT][2], o[NT][8][4];
+    // m: running maximum of s, mv: of s + lv; o in units of 2^mv.
+    float m[NT][2], mv[NT][2], l[NT][2], o[NT][8][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) m[t][x] = -INFINITY, l[t][x] = 0.f;
+      for (int x = 0; x < 2; ++x) m[t][x] = mv[t][x] = -INFINITY, l[t][x] = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -412,8 +448,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_ke
     const int stop = min(end, seq_end);
     for (; u < stop; ++u) {
       // ---- S^T = K Q^T
-      cp_wait<2>();
-      __syncwarp();
+      if (!mbar_wait(&sh.full[warp][slot], parity)) {
+        if (lane == 0) atomicOr(p.errors, 1);
+        return;
+      }
       float s[2][NT][4];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
@@ -421,36 +459,43 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_ke
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int x = 0; x < 4; ++x) s[mt][t][x] = 0.f;
-      const uint32_t kbase = smem_u32(ring[slot].rows) + rr * kBlockHeadDim;
-      const int ksw = row_swizzle(rr);
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      {
+        const int row = tile_row(rr);
+        const uint8_t* kbase = sh.rows[warp][slot] + row * kBlockHeadDim;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t at = kbase + mt * 16 * kBlockHeadDim + (((c + 4 * i) ^ ksw) << 4);
-          const uint4 ka = lds128(at), kb = lds128(at + 8 * kBlockHeadDim);
-          const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+          const uint8_t* at = kbase + (((c + 4 * i) ^ row) << 4);
+          uint4 k[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) k[x] = *reinterpret_cast<const uint4*>(at + 8 * x * kBlockHeadDim);
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t a0 = e4m3_to_f16x2(uint16_t(wa[w])), a2 = e4m3_to_f16x2(uint16_t(wa[w] >> 16));
-            const uint32_t a1 = e4m3_to_f16x2(uint16_t(wb[w])), a3 = e4m3_to_f16x2(uint16_t(wb[w] >> 16));
+            auto word = [&](int x) { return w == 0 ? k[x].x : w == 1 ? k[x].y : w == 2 ? k[x].z : k[x].w; };
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_f16(s[mt][t], a0, a1, a2, a3, qf[t][4 * i + w][0], qf[t][4 * i + w][1]);
+            for (int mt = 0; mt < 2; ++mt) {
+              const uint32_t wa = word(2 * mt), wb = word(2 * mt + 1);
+              const uint32_t a0 = e4m3_to_f16x2(uint16_t(wa)), a2 = e4m3_to_f16x2(uint16_t(wa >> 16));
+              const uint32_t a1 = e4m3_to_f16x2(uint16_t(wb)), a3 = e4m3_to_f16x2(uint16_t(wb >> 16));
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma_f16(s[mt][t], a0, a1, a2, a3, qf[t][4 * i + w][0], qf[t][4 * i + w][1]);
+            }
           }
         }
       }
-      const float ks = ring[slot].scale;
-      const int valid = ring[slot].valid;
-      __syncwarp();
-      ld.load(p, p.v_cache, p.v_scales, h, ring + slot, lane);  // V of the next tile
-      ld.next(p, prefix);
-      slot = slot == kSlots - 1 ? 0 : slot + 1;
+      const float ks = sh.scale[warp][slot];
+      const int valid = sh.valid[warp][slot];
+      advance();
 
-      // ---- softmax of the tile against its own maximum
+      // ---- softmax
+      if (!mbar_wait(&sh.full[warp][slot], parity)) {
+        if (lane == 0) atomicOr(p.errors, 1);
+        return;
+      }
+      const float lv = __log2f(sh.scale[warp][slot]);
       uint32_t pf[NT][2][2];
-      float alpha[NT][2], beta[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
+        float grow[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const float f = ks * qs[t][x];
@@ -460,27 +505,34 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_ke
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               float& v = s[mt][t][2 * y + x];
-              v = mt * 16 + y * 8 + rr < valid ? v * f : -INFINITY;
+              v *= f;
+              if (valid < kTile && mt * 16 + y * 8 + tile_row(rr) >= valid) v = -INFINITY;
               mx = fmaxf(mx, v);
             }
 #pragma unroll
           for (int k = 4; k <= 16; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-          const float m2 = fmaxf(m[t][x], mx);
-          const float ref = mx == -INFINITY ? 0.f : mx, ref2 = m2 == -INFINITY ? 0.f : m2;
-          alpha[t][x] = ex2(m[t][x] - ref2);
-          beta[t][x] = ex2(mx - ref2);
+          const float m2 = fmaxf(m[t][x], mx), mv2 = fmaxf(mv[t][x], mx + lv);
+          const float ref = m2 == -INFINITY ? 0.f : m2, refv = mv2 == -INFINITY ? 0.f : mv2;
+          grow[x] = ex2(mv[t][x] - refv);
           float sum = 0.f;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               float& v = s[mt][t][2 * y + x];
-              v = ex2(v - ref);
-              sum += v;
+              sum += ex2(v - ref);
+              v = ex2(v + (lv - refv));
             }
-          // A tile without a finite score: its exponentials are 0, or NaN if a score is.
-          l[t][x] = fmaf(l[t][x], alpha[t][x], mx == -INFINITY ? sum : sum * beta[t][x]);
+          l[t][x] = fmaf(l[t][x], ex2(m[t][x] - ref), sum);
+          if (mv2 == mv[t][x]) grow[x] = 1.f;
           m[t][x] = m2;
+          mv[t][x] = mv2;
+        }
+        if (__any_sync(0xffffffffu, grow[0] != 1.f || grow[1] != 1.f)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[t][j][x] *= grow[x & 1];
         }
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
@@ -489,52 +541,33 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_ke
       }
 
       // ---- O^T += V^T P^T
-      cp_wait<2>();
-      __syncwarp();
-      const uint32_t vbase = smem_u32(ring[slot].rows);
-      uint4 v[2][4];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < 2; ++mt) {
+        uint4 v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int row = mt * 16 + 2 * c + (k & 1) + (k >> 1) * 8;
-          v[mt][k] = lds128(vbase + row * kBlockHeadDim + ((rr ^ row_swizzle(row)) << 4));
+          const int row = mt * 16 + (k >> 1) * 8 + tile_row(2 * c + (k & 1));
+          v[k] = *reinterpret_cast<const uint4*>(sh.rows[warp][slot] + row * kBlockHeadDim + ((rr ^ (row & 7)) << 4));
+          if (valid < kTile && row >= valid) v[k] = make_uint4(0, 0, 0, 0);  // 0 x what lies there may be NaN
         }
-      const float vs = ring[slot].scale;
-      __syncwarp();
-      ld.load(p, p.k_cache, p.k_scales, h, ring + slot, lane);  // K of the tile after the next
-      slot = slot == kSlots - 1 ? 0 : slot + 1;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) beta[t][0] *= vs, beta[t][1] *= vs;
+        for (int w = 0; w < 4; ++w) {
+          auto word = [&](int k) { return w == 0 ? v[k].x : w == 1 ? v[k].y : w == 2 ? v[k].z : v[k].w; };
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t sel = half ? 0x7362u : 0x5140u;
-          float acc[NT][4];
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) acc[t][x] = 0.f;
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-            auto word = [&](int k) { return w == 0 ? v[mt][k].x : w == 1 ? v[mt][k].y : w == 2 ? v[mt][k].z : v[mt][k].w; };
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7362u : 0x5140u;
             const uint32_t e = __byte_perm(word(0), word(1), sel), f = __byte_perm(word(2), word(3), sel);
             const uint32_t a0 = e4m3_to_f16x2(uint16_t(e)), a1 = e4m3_to_f16x2(uint16_t(e >> 16));
             const uint32_t a2 = e4m3_to_f16x2(uint16_t(f)), a3 = e4m3_to_f16x2(uint16_t(f >> 16));
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_f16(acc[t], a0, a1, a2, a3, pf[t][mt][0], pf[t][mt][1]);
+            for (int t = 0; t < NT; ++t) mma_f16(o[t][2 * w + half], a0, a1, a2, a3, pf[t][mt][0], pf[t][mt][1]);
           }
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              o[t][2 * w + half][x] = fmaf(acc[t][x], beta[t][x & 1], o[t][2 * w + half][x] * alpha[t][x & 1]);
         }
       }
+      advance();
     }
 
-    // ---- the sequence (or its part in this range) is done
+    // ---- the sequence (or its part in this range) is done: o in units of 2^m
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -548,7 +581,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_ke
         for (int x = 0; x < 2; ++x) {
           const int g = t * 8 + 2 * c + x;
           if (g >= p.group) continue;
-          const float inv = l[t][x] == 0.f ? 0.f : 1.f / l[t][x];
+          const float inv = l[t][x] == 0.f ? 0.f : unit(mv[t][x], m[t][x]) / l[t][x];
           uint32_t w[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -567,10 +600,11 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_ke
         for (int x = 0; x < 2; ++x) {
           const int g = t * 8 + 2 * c + x;
           if (g >= p.group) continue;
+          const float f = unit(mv[t][x], m[t][x]);
           float4* dst = reinterpret_cast<float4*>(p.part_o + (part + g) * kBlockHeadDim + 16 * rr);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            __stcg(dst + j, make_float4(o[t][2 * j][x], o[t][2 * j][2 + x], o[t][2 * j + 1][x], o[t][2 * j + 1][2 + x]));
+            __stcg(dst + j, make_float4(o[t][2 * j][x] * f, o[t][2 * j][2 + x] * f, o[t][2 * j + 1][x] * f, o[t][2 * j + 1][2 + x] * f));
           if (rr == 0) __stcg(&p.part_ml[part + g], make_float2(m[t][x], l[t][x]));
         }
       const int first = range_of(seq_begin), last = range_of(seq_end - 1), parts = last - first + 1;
@@ -589,13 +623,33 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) decode_blocks_ke
     }
     do ++b; while (u < end && prefix[b + 1] == u);
   }
-  cp_wait<0>();
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+bool encode_cache_map(CUtensorMap* map, const void* cache, int64_t rows, int num_kv_heads) {
+  static const EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeTiledFn>(ptr)
+               : nullptr;
+  }();
+  const cuuint64_t row_bytes = cuuint64_t(num_kv_heads) * kBlockHeadDim;
+  const cuuint64_t dims[2] = {row_bytes, cuuint64_t(rows)}, strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {kBlockHeadDim, kTile}, steps[2] = {1, 1};
+  return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int NT>
 int launch_decode_blocks(const BlockDecodeParams& p, cudaStream_t s) {
   constexpr int kPerSm = NT == 1 ? 2 : 1;
-  constexpr int kSlotBytes = int(sizeof(Slot)) * kSlots * kWarps;
+  constexpr int kShared = int(sizeof(Shared));
   static std::atomic<int> sms[kMaxDevices];  // 0: this kernel is not set up on the device yet
   int dev = -1;
   cudaError_t e = cudaGetDevice(&dev);
@@ -604,7 +658,7 @@ int launch_decode_blocks(const BlockDecodeParams& p, cudaStream_t s) {
     e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(decode_blocks_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kSlotBytes + 4 * (kMaxBatch + 1));
+                               kShared + 4 * (kMaxBatch + 1));
     if (e == cudaSuccess && dev < kMaxDevices) sms[dev].store(n, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) {
@@ -613,7 +667,7 @@ int launch_decode_blocks(const BlockDecodeParams& p, cudaStream_t s) {
   }
   int ctas = n * kPerSm < kMaxCtas ? n * kPerSm : kMaxCtas;
   if (ctas * kWarps < p.num_kv_heads) ctas = (p.num_kv_heads + kWarps - 1) / kWarps;
-  decode_blocks_kernel<NT><<<ctas, 32 * kWarps, kSlotBytes + 4 * (p.batch + 1), s>>>(p);
+  decode_blocks_kernel<NT><<<ctas, 32 * (kWarps + 1), kShared + 4 * (p.batch + 1), s>>>(p);
   HL_CHECK_LAUNCH("hl_paged_decode_fp8_blocks");
   return HL_OK;
 }
@@ -653,6 +707,7 @@ extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, c
   HL_CHECK_ARG(int64_t(max_blocks_per_seq) * block_size <= 0x7fffffff &&
                    int64_t(batch) * max_blocks_per_seq * (block_size / kTile) <= 0x7fffffff,
                "hl_paged_decode_fp8_blocks: the block tables span 2^31 tokens a row or 2^36 in all");
+  HL_CHECK_ARG(num_blocks <= 0x7fffffff / block_size, "hl_paged_decode_fp8_blocks: a pool of 2^31 tokens or more");
   HL_CHECK_ARG(num_kv_heads <= kMaxRanges, "hl_paged_decode_fp8_blocks: more than %d KV heads", kMaxRanges);
   HL_CHECK_ARG(aligned16(q) && q_row_stride % 8 == 0 && q_row_stride >= int64_t(num_q_heads) * head_dim &&
                    aligned16(out) && out_row_stride % 8 == 0 && out_row_stride >= int64_t(num_q_heads) * head_dim &&
@@ -667,8 +722,11 @@ extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, c
   BlockDecodeParams p;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_stride = q_row_stride;
-  p.k_cache = static_cast<const uint8_t*>(k_cache);
-  p.v_cache = static_cast<const uint8_t*>(v_cache);
+  if (!encode_cache_map(&p.k_map, k_cache, num_blocks * block_size, num_kv_heads) ||
+      !encode_cache_map(&p.v_map, v_cache, num_blocks * block_size, num_kv_heads)) {
+    set_error("hl_paged_decode_fp8_blocks: cuTensorMapEncodeTiled failed");
+    return HL_ERR_CUDA;
+  }
   p.k_scales = k_scales;
   p.v_scales = v_scales;
   p.block_tables = block_tables;
