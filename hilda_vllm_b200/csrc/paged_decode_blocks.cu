@@ -21,12 +21,14 @@
 // fp32 2^(s - m): scales of any range cost no precision, and the f16 rounding (2^-12) is relative to
 // the largest weighted value.  Maxima, sums and outputs are fp32; O is rescaled only when M grows.
 //
-// Work split: the tiles of all sequences in a row are cut into equal ranges, one per warp and head
-// (Hk neighbouring warps read the Hk heads of the same tokens, a contiguous piece of the cache).  A
-// sequence inside one range is written out directly; the parts of one cut across ranges go to the
-// workspace and the warp that finishes last merges them in range order (tickets; results do not
-// depend on the order of arrival).  More than kMergeFan parts are merged in two levels, so that the
-// ~300 parts of one long sequence are not read by a single warp.
+// Work split: a thread block serves one KV head (neighbouring blocks the Hk heads of the same
+// tokens).  The tiles of all sequences, with one unit of cost more per sequence for its queries and
+// result, form a row that is cut into equal ranges, one per warp and eight per block.  A sequence
+// inside one warp's range is written out directly; one cut between warps leaves a part per warp in
+// the workspace (L2), and the warp that finishes last (a ticket, in shared memory where the block has
+// all parts) merges them in order, so results do not depend on the order of arrival.  A sequence of
+// more than kDirectMerge parts is merged by whole blocks, to one part per block first, and more than
+// kFlatMerge of those in two levels, so that no warp reads many parts one after another.
 #include "kv_blocks.cuh"
 
 #include <cuda.h>
@@ -43,8 +45,10 @@ constexpr int kTile = 32;                           // tokens of one tile
 constexpr int kTileBytes = kTile * kBlockHeadDim;   // one ring slot
 constexpr int kSlots = 3;
 constexpr int kMaxCtas = 296;                       // two per SM of a B200
-constexpr int kMaxRanges = kMaxCtas * kWarps;       // (range, head) pairs at most
-constexpr int kMergeFan = 16;
+constexpr int kDirectMerge = 16;                    // warps' parts merged by one warp
+constexpr int kFlatMerge = 40;
+constexpr int kMinUnits = 2;                        // of a range: shorter ones cost more in merging
+constexpr int kMergeFan = 16;                       // parts of a first-level group
 constexpr int kMaxDevices = 64;
 
 struct BlockDecodeParams {
@@ -64,23 +68,27 @@ struct BlockDecodeParams {
   __nv_bfloat16* out;
   int64_t out_stride;
   int32_t* errors;
-  int32_t* tickets;      // [batch][Hk], all parts of a sequence
-  int32_t* sub_tickets;  // [2 * ranges][Hk], one group of kMergeFan parts
-  float2* part_ml;       // [2 * ranges][Hk][G]: (m, l)
-  float* part_o;         // [2 * ranges][Hk][G][128]
+  int32_t* tickets;      // [kMaxCtas]: the blocks of the sequence that goes on behind a block
+  int32_t* sub_tickets;  // [2 * kMaxCtas]: a group of kMergeFan blocks, by its first part
+  // Parts of (range, head), then of (block, head), two each (slot 0: of a sequence that began before,
+  // 1: of one that goes on behind): [2 * kMaxCtas * (kWarps + 1)][G], o also [128]; o in units of 2^m.
+  float2* part_ml;       // (m, l)
+  float* part_o;
 };
+
+constexpr int kWarpParts = 2 * kMaxCtas * kWarps;
 
 // Workspace: error word | tickets | sub-tickets | (m, l) | o.
 struct WsLayout {
   int64_t sub, ml, o, end;
 };
-__host__ __device__ inline WsLayout ws_layout(int batch, int num_q_heads, int num_kv_heads) {
-  const int64_t parts = 2 * int64_t(kMaxRanges / num_kv_heads);
+__host__ __device__ inline WsLayout ws_layout(int group) {
+  const int64_t rows = int64_t(kWarpParts + 2 * kMaxCtas) * group;
   WsLayout w;
-  w.sub = 256 + (int64_t(batch) * num_kv_heads * 4 + 255) / 256 * 256;
-  w.ml = w.sub + (parts * num_kv_heads * 4 + 255) / 256 * 256;
-  w.o = w.ml + (parts * num_q_heads * 8 + 255) / 256 * 256;
-  w.end = w.o + parts * num_q_heads * kBlockHeadDim * 4;
+  w.sub = 256 + kMaxCtas * 4;
+  w.ml = (w.sub + 2 * kMaxCtas * 4 + 255) / 256 * 256;
+  w.o = w.ml + (rows * 8 + 255) / 256 * 256;
+  w.end = w.o + rows * kBlockHeadDim * 4;
   return w;
 }
 
@@ -144,15 +152,16 @@ struct Shared {
   float scale[kWarps][kSlots];
   int32_t valid[kWarps][kSlots];  // tokens the tile holds; 0: its page is outside the pool
   int32_t warp_sum[kWarps + 1];
-  int32_t pad;
-  int32_t prefix[];  // [batch + 1] first tile of each sequence
+  int32_t last;             // broadcast of a ticket
+  int32_t tickets[kWarps];  // sequences that begin in a warp's range and end in another's of the block
+  int32_t prefix[];  // [batch + 1] first unit of each sequence: its cost unit, then its tiles
 };
 
-// The producer lane of one consumer warp: walks the tiles [u, end) and copies K, then V of each into
-// the next ring slot that is empty.
+// The producer lane of one consumer warp: walks the tiles of the units [u, end) and copies K, then V
+// of each into the next ring slot that is empty.
 struct Loader {
-  int u, end;      // next tile, end of the range
-  int b, b_end;    // its sequence, and that sequence's first tile index behind it
+  int u, end;      // next unit (a tile's), end of the range
+  int b, b_end;    // its sequence, and the first unit behind it
   int n;           // tokens left in the sequence from this tile on
   int page_at, off, group_off, group;  // table index, token offset in the page, in its group; group in the page
   int page;        // block id, or -1
@@ -165,7 +174,8 @@ struct Loader {
     }
   }
   __device__ __forceinline__ void enter(const BlockDecodeParams& p, const int* prefix) {
-    const int tok = (u - prefix[b]) * kTile;
+    if (u == prefix[b] && ++u >= end) return;  // the cost unit
+    const int tok = (u - prefix[b] - 1) * kTile;
     n = min(p.context_lens[b], p.max_blocks * p.block_size) - tok;
     b_end = prefix[b + 1];
     page_at = tok / p.block_size;
@@ -209,74 +219,153 @@ struct Loader {
   }
 };
 
-// (m, l, o) of `count` parts first, first + step, ... of one (sequence, head), merged in that order into
-// out (bf16, when final) or back into part `first`.
-__device__ void merge_parts(const BlockDecodeParams& p, int h, int first_slot, int first, int step, int count, int b,
-                            bool final, int lane) {
-  for (int g = 0; g < p.group; ++g) {
-    auto index = [&](int i) {  // part i of the list
-      const int r = first + i * step;
-      const int slot = r == first && first_slot ? 2 * r + 1 : 2 * r;
-      return (int64_t(slot) * p.num_kv_heads + h) * p.group + g;
-    };
-    float mm = -INFINITY;
-    for (int i = lane; i < count; i += 32) mm = fmaxf(mm, __ldcg(&p.part_ml[index(i)]).x);
+struct Merged {
+  float m, l;
+  float4 o;
+};
+
+// (m, l, o) of one head over `count` parts, the first at index `first`, the i-th at rest + i * stride,
+// summed in that order; a lane holds four dimensions.  All loads of up to 16 parts are in flight
+// together; a call of its own, so that they take no registers from the tile loop.
+__device__ __noinline__ Merged merge_parts(const float2* __restrict__ part_ml, const float* __restrict__ part_o,
+                                           int count, int first, int rest, int stride, int lane) {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto index = [&](int i) { return i == 0 ? first : rest + i * stride; };
+  for (int i0 = 0; i0 < count; i0 += 16) {
+    const int i = i0 + (lane & 15);
+    const float2 ml = i < count ? __ldcg(part_ml + index(i)) : make_float2(-INFINITY, 0.f);
+    float4 v[16];
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    const float ref = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < count; i0 += 32) {
-      float w = 0.f, wl = 0.f;
-      if (i0 + lane < count) {
-        const float2 ml = __ldcg(&p.part_ml[index(i0 + lane)]);
-        w = ex2(ml.x - ref);
-        wl = w * ml.y;
-      }
+    for (int k = 0; k < 16; ++k)
+      v[k] = i0 + k < count ? __ldcg(reinterpret_cast<const float4*>(part_o + int64_t(index(i0 + k)) * kBlockHeadDim) + lane)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+    float mx = ml.x;
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) wl += __shfl_xor_sync(0xffffffffu, wl, o);
-      ll += wl;
-      const int k = min(32, count - i0);
-#pragma unroll 8
-      for (int i = 0; i < k; ++i) {
-        const float wi = __shfl_sync(0xffffffffu, w, i);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + index(i0 + i) * kBlockHeadDim) + lane);
-        acc.x = fmaf(v.x, wi, acc.x);
-        acc.y = fmaf(v.y, wi, acc.y);
-        acc.z = fmaf(v.z, wi, acc.z);
-        acc.w = fmaf(v.w, wi, acc.w);
-      }
-    }
-    if (final) {
-      const float inv = ll == 0.f ? 0.f : 1.f / ll;
-      const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv);
-      const __nv_bfloat162 hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(p.out + b * p.out_stride + (int64_t(h) * p.group + g) * kBlockHeadDim + 4 * lane) =
-          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-    } else {
-      const int64_t at = index(0);
-      __syncwarp();
-      __stcg(reinterpret_cast<float4*>(p.part_o + at * kBlockHeadDim) + lane, acc);
-      if (lane == 0) __stcg(&p.part_ml[at], make_float2(mm, ll));
+    for (int k = 8; k >= 1; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+    mx = fmaxf(m, mx);
+    const float ref = mx == -INFINITY ? 0.f : mx, keep = ex2(m - ref), w = ex2(ml.x - ref);
+    float wl = w * ml.y;
+#pragma unroll
+    for (int k = 8; k >= 1; k >>= 1) wl += __shfl_xor_sync(0xffffffffu, wl, k);
+    m = mx;
+    l = fmaf(l, keep, wl);
+    o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      o.x = fmaf(v[k].x, wk, o.x);
+      o.y = fmaf(v[k].y, wk, o.y);
+      o.z = fmaf(v[k].z, wk, o.z);
+      o.w = fmaf(v[k].w, wk, o.w);
     }
   }
+  return Merged{m, l, o};
+}
+
+// One sequence's `count` <= 16 parts of all G heads, merged in order and written to `out` by one warp:
+// four parts of four heads are in flight together.
+__device__ __noinline__ void merge_and_write(const float2* __restrict__ part_ml, const float* __restrict__ part_o,
+                                             int count, int first, int rest, int stride, int group,
+                                             __nv_bfloat16* __restrict__ out, int lane) {
+  for (int g0 = 0; g0 < group; g0 += 4) {
+    // Lane: part lane % 16, heads g0 + 2 (lane / 16) and the next.
+    const int i = lane & 15, gl = g0 + 2 * (lane >> 4);
+    float w[2], l[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float2 ml = i < count && gl + x < group ? __ldcg(part_ml + (i == 0 ? first : rest + i * stride) + gl + x)
+                                                    : make_float2(-INFINITY, 0.f);
+      w[x] = ml.x;
+      l[x] = ml.y;
+    }
+    float4 o[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < count; i0 += 4) {
+      float4 v[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          v[k][g] = i0 + k < count && g0 + g < group
+                        ? __ldcg(reinterpret_cast<const float4*>(
+                                     part_o + int64_t((i0 + k == 0 ? first : rest + (i0 + k) * stride) + g0 + g) * kBlockHeadDim) +
+                                 lane)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 == 0) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float m = w[x];
+#pragma unroll
+          for (int k = 8; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+          w[x] = ex2(w[x] - (m == -INFINITY ? 0.f : m));
+          l[x] *= w[x];
+#pragma unroll
+          for (int k = 8; k >= 1; k >>= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], k);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float wk = __shfl_sync(0xffffffffu, w[g & 1], 16 * (g >> 1) + ((i0 + k) & 15));
+          o[g].x = fmaf(v[k][g].x, wk, o[g].x);
+          o[g].y = fmaf(v[k][g].y, wk, o[g].y);
+          o[g].z = fmaf(v[k][g].z, wk, o[g].z);
+          o[g].w = fmaf(v[k][g].w, wk, o[g].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float sum = __shfl_sync(0xffffffffu, l[g & 1], 16 * (g >> 1));
+      if (g0 + g >= group) continue;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(o[g].x * inv, o[g].y * inv);
+      const __nv_bfloat162 hi = __floats2bfloat162_rn(o[g].z * inv, o[g].w * inv);
+      *reinterpret_cast<uint2*>(out + (g0 + g) * kBlockHeadDim + 4 * lane) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+  }
+}
+
+__device__ __forceinline__ void write_part(const BlockDecodeParams& p, int at, int lane, const Merged& r) {
+  __stcg(reinterpret_cast<float4*>(p.part_o + int64_t(at) * kBlockHeadDim) + lane, r.o);
+  if (lane == 0) __stcg(&p.part_ml[at], make_float2(r.m, r.l));
+}
+
+__device__ __forceinline__ void write_row(const BlockDecodeParams& p, int b, int head, int lane, const Merged& r) {
+  const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(r.o.x * inv, r.o.y * inv);
+  const __nv_bfloat162 hi = __floats2bfloat162_rn(r.o.z * inv, r.o.w * inv);
+  *reinterpret_cast<uint2*>(p.out + b * p.out_stride + head * kBlockHeadDim + 4 * lane) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 
 // 2^(mv - m), the factor from units of 2^mv to units of 2^m; 0 where nothing was summed.
 __device__ __forceinline__ float unit(float mv, float m) { return mv == -INFINITY ? 0.f : exp2f(mv - m); }
 
-// True for the warp that takes the last of `count` tickets; it leaves the counter at zero.
-__device__ __forceinline__ bool last_ticket(int32_t* ticket, int count, int lane) {
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
+
+// All consumer warps of the block: true if the block took the last of `count` tickets, after which
+// the other blocks' parts can be read.  The counter is left at zero.
+__device__ __forceinline__ bool block_is_last(Shared& sh, int32_t* ticket, int count) {
   __threadfence();
-  __syncwarp();
-  int last = 0;
-  if (lane == 0) {
-    last = atomicAdd(ticket, 1) == count - 1;
+  consumers_sync();
+  if (threadIdx.x == 0) {
+    const int last = atomicAdd(ticket, 1) == count - 1;
     if (last) *ticket = 0;
+    __threadfence();
+    sh.last = last;
   }
-  last = __shfl_sync(0xffffffffu, last, 0);
-  if (last) __threadfence();
-  return last;
+  consumers_sync();
+  return sh.last;
+}
+
+__device__ __forceinline__ int units_of(int context, int width) {
+  const int n = min(context, width);
+  return n <= 0 ? 0 : 1 + (n + kTile - 1) / kTile;
 }
 
 template <int NT>
@@ -286,18 +375,19 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
   Shared& sh = *reinterpret_cast<Shared*>(smem);
   int* prefix = sh.prefix;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < kWarps) sh.tickets[threadIdx.x] = 0;
   if (threadIdx.x < kWarps * kSlots) {
     mbar_init(&sh.full[0][0] + threadIdx.x, 2);   // the tile's bytes and the scale
     mbar_init(&sh.empty[0][0] + threadIdx.x, 1);
     fence_mbar_init();
   }
-  // Tiles of each sequence and their prefix sums.
+  // Units of each sequence and their prefix sums.
   {
     constexpr int kThreads = 32 * (kWarps + 1);
     const int per = (p.batch + kThreads - 1) / kThreads, width = p.max_blocks * p.block_size;
     const int b0 = threadIdx.x * per;
     int sum = 0;
-    for (int b = b0; b < min(b0 + per, p.batch); ++b) sum += (max(min(p.context_lens[b], width), 0) + kTile - 1) / kTile;
+    for (int b = b0; b < min(b0 + per, p.batch); ++b) sum += units_of(p.context_lens[b], width);
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -310,15 +400,21 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
     for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
     for (int b = b0; b < min(b0 + per, p.batch); ++b) {
       prefix[b] = before;
-      before += (max(min(p.context_lens[b], width), 0) + kTile - 1) / kTile;
+      before += units_of(p.context_lens[b], width);
       if (b == p.batch - 1) prefix[p.batch] = before;
     }
     __syncthreads();
   }
   const int total = prefix[p.batch];
-  const int ranges = min(int(gridDim.x) * kWarps / p.num_kv_heads, total);
-  auto range_begin = [&](int r) { return int(int64_t(r) * total / ranges); };
-  auto range_of = [&](int u) { return int((int64_t(u) * ranges + ranges - 1) / total); };  // that tile u lies in
+  const int h = blockIdx.x % p.num_kv_heads, block = blockIdx.x / p.num_kv_heads, base = block * kWarps;
+  const int ranges = min(int(gridDim.x) / p.num_kv_heads * kWarps, (total + kMinUnits - 1) / kMinUnits);
+  // Ranges of `share` units, the first `more` of them of one more.
+  const unsigned share = unsigned(total) / max(ranges, 1), more = unsigned(total) - share * ranges;
+  auto range_begin = [&](int r) { return int(r * share + min(unsigned(r), more)); };
+  auto range_of = [&](unsigned u) {  // that unit u lies in
+    const unsigned wide = more * (share + 1);
+    return int(u < wide ? u / (share + 1) : more + (u - wide) / share);
+  };
   auto sequence_of = [&](int u) {  // the last sequence that begins at or before u: it has tiles
     int lo = 0, hi = p.batch - 1;
     while (lo < hi) {
@@ -330,8 +426,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
 
   if (warp == kWarps) {
     // ---- producer: lane w loads for warp w
-    const int gid = blockIdx.x * kWarps + lane;
-    const int h = gid % p.num_kv_heads, range = gid / p.num_kv_heads;
+    const int range = base + lane;
     Loader ld;
     ld.u = ld.end = 0;
     if (lane < kWarps && range < ranges) {
@@ -375,13 +470,12 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
     uint4* o = reinterpret_cast<uint4*>(p.out + b * p.out_stride);
     for (int i = threadIdx.x; i < p.group * p.num_kv_heads * (kBlockHeadDim / 8); i += 32 * kWarps) o[i] = make_uint4(0, 0, 0, 0);
   }
-  const int gid = blockIdx.x * kWarps + warp;
-  const int h = gid % p.num_kv_heads, range = gid / p.num_kv_heads;
-  if (range >= ranges) return;
-  int u = range_begin(range);
-  const int end = range_begin(range + 1);
-  int b = sequence_of(u);
+  const int range = base + warp;
+  int u = range < ranges ? range_begin(range) : 0;
+  const int end = range < ranges ? range_begin(range + 1) : 0;
+  int b = u < end ? sequence_of(u) : 0;
 
+  const int part_stride = 2 * p.num_kv_heads * p.group;  // from one range's (or block's) parts to the next's
   const int c = lane & 3, rr = lane >> 2;
   int slot = 0;
   uint32_t parity = 0;
@@ -391,6 +485,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
     if (++slot == kSlots) slot = 0, parity ^= 1;
   };
   while (u < end) {
+    if (u == prefix[b] && ++u >= end) break;  // the cost unit
     // ---- one sequence: its query heads as B fragments
     uint32_t qf[NT][8][2];
     float qs[NT][2];
@@ -444,13 +539,14 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
         for (int x = 0; x < 4; ++x) o[t][j][x] = 0.f;
     }
     const int seq_end = prefix[b + 1], seq_begin = prefix[b];
-    const bool begins = u == seq_begin;
+    const bool begins = u == seq_begin + 1;
     const int stop = min(end, seq_end);
     for (; u < stop; ++u) {
       // ---- S^T = K Q^T
       if (!mbar_wait(&sh.full[warp][slot], parity)) {
         if (lane == 0) atomicOr(p.errors, 1);
-        return;
+        u = end;
+        break;
       }
       float s[2][NT][4];
 #pragma unroll
@@ -489,7 +585,8 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
       // ---- softmax
       if (!mbar_wait(&sh.full[warp][slot], parity)) {
         if (lane == 0) atomicOr(p.errors, 1);
-        return;
+        u = end;
+        break;
       }
       const float lv = __log2f(sh.scale[warp][slot]);
       uint32_t pf[NT][2][2];
@@ -593,7 +690,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
           dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
         }
     } else {
-      const int64_t part = (int64_t(2 * range + (begins ? 1 : 0)) * p.num_kv_heads + h) * p.group;
+      const int part = (2 * (range * p.num_kv_heads + h) + (begins ? 1 : 0)) * p.group;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -601,27 +698,76 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
           const int g = t * 8 + 2 * c + x;
           if (g >= p.group) continue;
           const float f = unit(mv[t][x], m[t][x]);
-          float4* dst = reinterpret_cast<float4*>(p.part_o + (part + g) * kBlockHeadDim + 16 * rr);
+          float4* dst = reinterpret_cast<float4*>(p.part_o + int64_t(part + g) * kBlockHeadDim + 16 * rr);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             __stcg(dst + j, make_float4(o[t][2 * j][x] * f, o[t][2 * j][2 + x] * f, o[t][2 * j + 1][x] * f, o[t][2 * j + 1][2 + x] * f));
           if (rr == 0) __stcg(&p.part_ml[part + g], make_float2(m[t][x], l[t][x]));
         }
-      const int first = range_of(seq_begin), last = range_of(seq_end - 1), parts = last - first + 1;
-      int32_t* ticket = p.tickets + int64_t(b) * p.num_kv_heads + h;
-      if (parts <= kMergeFan) {
-        if (last_ticket(ticket, parts, lane)) merge_parts(p, h, 1, first, 1, parts, b, true, lane);
-      } else {
-        const int sub = (range - first) / kMergeFan, subs = (parts + kMergeFan - 1) / kMergeFan;
-        const int head = first + sub * kMergeFan, count = min(kMergeFan, last - head + 1);
-        const int head_slot = 2 * head + (sub == 0 ? 1 : 0);
-        if (last_ticket(p.sub_tickets + int64_t(head_slot) * p.num_kv_heads + h, count, lane)) {
-          merge_parts(p, h, sub == 0, head, 1, count, b, false, lane);
-          if (last_ticket(ticket, subs, lane)) merge_parts(p, h, 1, first, kMergeFan, subs, b, true, lane);
+      // The last warp of a sequence of few parts merges them.
+      const int first = range_of(seq_begin + 1), last = range_of(seq_end - 1), parts = last - first + 1;
+      if (parts <= kDirectMerge) {
+        const bool own = first >= base && last < base + kWarps;
+        if (own) __threadfence_block(); else __threadfence();
+        __syncwarp();
+        int done = 0;
+        if (lane == 0) {
+          if (own) {
+            done = atomicAdd(&sh.tickets[first - base], 1) == parts - 1;
+          } else {  // one arrival per warp; left at zero for the next launch
+            int32_t* ticket = p.tickets + first / kWarps * p.num_kv_heads + h;
+            done = atomicAdd(ticket, 1) == parts - 1;
+            if (done) *ticket = 0;
+          }
+        }
+        if (__shfl_sync(0xffffffffu, done, 0)) {
+          if (own) __threadfence_block(); else __threadfence();
+          const int from = 2 * (first * p.num_kv_heads + h) * p.group;
+          merge_and_write(p.part_ml, p.part_o, parts, from + p.group, from, part_stride, p.group,
+                          p.out + b * p.out_stride + int64_t(h) * p.group * kBlockHeadDim, lane);
         }
       }
     }
     do ++b; while (u < end && prefix[b + 1] == u);
+  }
+
+  // ---- long sequences, which are cut at this block's first border (they came in), its last (they go
+  // on), or both
+  if (base >= ranges) return;
+  for (int side = 0; side < 2; ++side) {
+    const int border = range_begin(min(base + side * kWarps, ranges));
+    if (border >= total) continue;
+    const int b = sequence_of(border);
+    if (border <= prefix[b] + 1) continue;  // no tile of it lies in front
+    const int first = range_of(prefix[b] + 1), last = range_of(prefix[b + 1] - 1);
+    if (last - first < kDirectMerge || (side && first < base)) continue;
+    consumers_sync();  // the block's parts are written
+    const int k0 = first / kWarps, k1 = last / kWarps;
+    // Part of block k: slot 1 where the sequence begins, 0 behind it.
+    auto at_rest = [&](int k, int g) { return (kWarpParts + 2 * (k * p.num_kv_heads + h)) * p.group + g; };
+    auto at = [&](int k, int g) { return at_rest(k, g) + (k == k0 ? p.group : 0); };
+    const int w0 = max(first, base), w1 = min(last, base + kWarps - 1);
+    for (int g = warp; g < p.group; g += kWarps) {
+      const int from = 2 * (w0 * p.num_kv_heads + h) * p.group + g;
+      write_part(p, at(block, g), lane,
+                 merge_parts(p.part_ml, p.part_o, w1 - w0 + 1, w0 == first ? from + p.group : from, from, part_stride, lane));
+    }
+    int step = 1, count = k1 - k0 + 1;
+    if (count > kFlatMerge) {
+      const int head = k0 + (block - k0) / kMergeFan * kMergeFan, n = min(kMergeFan, k1 - head + 1);
+      if (!block_is_last(sh, p.sub_tickets + 2 * (head * p.num_kv_heads + h) + (head == k0), n)) continue;
+      for (int g = warp; g < p.group; g += kWarps) {
+        const Merged r = merge_parts(p.part_ml, p.part_o, n, at(head, g), at_rest(head, g), part_stride, lane);
+        write_part(p, at(head, g), lane, r);
+      }
+      step = kMergeFan;
+      count = (count + kMergeFan - 1) / kMergeFan;
+    }
+    if (!block_is_last(sh, p.tickets + k0 * p.num_kv_heads + h, count)) continue;
+    for (int g = warp; g < p.group; g += kWarps) {
+      write_row(p, b, h * p.group + g, lane,
+                merge_parts(p.part_ml, p.part_o, count, at(k0, g), at_rest(k0, g), step * part_stride, lane));
+    }
   }
 }
 
@@ -666,7 +812,7 @@ int launch_decode_blocks(const BlockDecodeParams& p, cudaStream_t s) {
     return HL_ERR_CUDA;
   }
   int ctas = n * kPerSm < kMaxCtas ? n * kPerSm : kMaxCtas;
-  if (ctas * kWarps < p.num_kv_heads) ctas = (p.num_kv_heads + kWarps - 1) / kWarps;
+  if (ctas < p.num_kv_heads) ctas = p.num_kv_heads;
   decode_blocks_kernel<NT><<<ctas, 32 * (kWarps + 1), kShared + 4 * (p.batch + 1), s>>>(p);
   HL_CHECK_LAUNCH("hl_paged_decode_fp8_blocks");
   return HL_OK;
@@ -679,8 +825,8 @@ using namespace hl;
 
 extern "C" int64_t hl_paged_decode_fp8_blocks_workspace_size(int batch, int num_q_heads, int num_kv_heads) {
   if (batch <= 0 || batch > kMaxBatch || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return -1;
-  if (num_kv_heads > kMaxRanges) return -1;
-  return ws_layout(batch, num_q_heads, num_kv_heads).end;
+  if (num_kv_heads > kMaxCtas) return -1;
+  return ws_layout(num_q_heads / num_kv_heads).end;
 }
 
 extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, const void* k_cache,
@@ -705,10 +851,10 @@ extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, c
   HL_CHECK_ARG(max_blocks_per_seq > 0 && bt_stride >= max_blocks_per_seq && num_blocks > 0,
                "hl_paged_decode_fp8_blocks: bad block table or pool shape");
   HL_CHECK_ARG(int64_t(max_blocks_per_seq) * block_size <= 0x7fffffff &&
-                   int64_t(batch) * max_blocks_per_seq * (block_size / kTile) <= 0x7fffffff,
+                   int64_t(batch) * max_blocks_per_seq * (block_size / kTile + 1) <= 0x7fffffff,
                "hl_paged_decode_fp8_blocks: the block tables span 2^31 tokens a row or 2^36 in all");
   HL_CHECK_ARG(num_blocks <= 0x7fffffff / block_size, "hl_paged_decode_fp8_blocks: a pool of 2^31 tokens or more");
-  HL_CHECK_ARG(num_kv_heads <= kMaxRanges, "hl_paged_decode_fp8_blocks: more than %d KV heads", kMaxRanges);
+  HL_CHECK_ARG(num_kv_heads <= kMaxCtas, "hl_paged_decode_fp8_blocks: more than %d KV heads", kMaxCtas);
   HL_CHECK_ARG(aligned16(q) && q_row_stride % 8 == 0 && q_row_stride >= int64_t(num_q_heads) * head_dim &&
                    aligned16(out) && out_row_stride % 8 == 0 && out_row_stride >= int64_t(num_q_heads) * head_dim &&
                    aligned16(k_cache) && aligned16(v_cache),
@@ -742,7 +888,7 @@ extern "C" int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, c
   p.out = static_cast<__nv_bfloat16*>(out);
   p.out_stride = out_row_stride;
   p.group = num_q_heads / num_kv_heads;
-  const WsLayout w = ws_layout(batch, num_q_heads, num_kv_heads);
+  const WsLayout w = ws_layout(p.group);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.errors = reinterpret_cast<int32_t*>(ws);
   p.tickets = reinterpret_cast<int32_t*>(ws + 256);
