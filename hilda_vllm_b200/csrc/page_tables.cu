@@ -8,13 +8,20 @@
 //   its need_b - have_b new pages are the next ones of free_blocks, sequence after sequence;
 //   token i of its n_b has position c_b + i and slot row[pos / BS] * BS + pos % BS.
 // Whole numbers only; the bytes are the token arrays (12 B a token) and the table rows.
+//
+// One launch.  Bound by latency up to some 100k tokens: lengths -> prefix sums -> free list or table ->
+// slots are three dependent reads.  So every thread block scans all lengths itself (at most 4096, from
+// L2) instead of waiting for one that does, and no thread reads a table entry that another writes: a
+// token on a new page takes the page's id from the free list, as the thread that writes the row does.
 #include "hl_common.cuh"
 
 namespace hl {
 namespace {
 
-constexpr int kTableThreads = 1024;
+constexpr int kTableThreads = 256;
+constexpr int kTokensPerThread = 4;
 constexpr int kMaxTableSeqs = 4096;
+constexpr int kMaxTableBlocks = 296;  // two per SM: more blocks would only repeat the scan
 
 struct TableParams {
   const int32_t* cached_lens;
@@ -33,75 +40,150 @@ struct TableParams {
   int64_t* positions;
   int32_t* slot_mapping;
   int32_t* status;
+  bool wide;  // positions and slot_mapping are aligned for 16-byte stores
 };
 
-__device__ __forceinline__ int64_t cached(const TableParams& p, int b) {
+__device__ __forceinline__ unsigned cached(const TableParams& p, int b) {
   return p.cached_lens ? max(p.cached_lens[b], 0) : 0;
 }
 
 // Pages of `tokens` tokens, cut at the width of a table row.
-__device__ __forceinline__ int64_t pages_of(const TableParams& p, int64_t tokens) {
-  const int64_t n = (tokens + p.block_size - 1) / p.block_size;
-  return n < p.max_blocks ? n : p.max_blocks;
+__device__ __forceinline__ unsigned pages_of(const TableParams& p, unsigned tokens) {
+  return min(tokens / p.block_size + (tokens % p.block_size != 0), unsigned(p.max_blocks));
 }
 
-// One thread block: prefix sums over the sequences, then the table rows.
-__global__ void __launch_bounds__(kTableThreads) extend_tables_kernel(const TableParams p) {
-  __shared__ int64_t s_start[kMaxTableSeqs];
-  __shared__ int s_err;
-  if (threadIdx.x == 0) {
-    s_err = 0;
-    int64_t q = 0, k = 0, pages = 0;
-    p.cu_seqlens_q[0] = 0;
-    p.cu_seqlens_k[0] = 0;
-    for (int b = 0; b < p.num_seqs; ++b) {
-      const int64_t c = cached(p, b), n = max(p.query_lens[b], 0);
-      const int64_t have = pages_of(p, c), need = n > 0 ? pages_of(p, c + n) : have;
-      s_start[b] = pages;
-      q += n;
-      k += c + n;
-      pages += need - have;
-      p.cu_seqlens_q[b + 1] = int32_t(q);
-      p.cu_seqlens_k[b + 1] = int32_t(k);
-      p.context_lens[b] = int32_t(c + n);
-      if (n > 0 && c + n > int64_t(p.max_blocks) * p.block_size) s_err |= HL_TABLES_TOO_NARROW;
+struct Sums {
+  int64_t query, context, pages;
+  __device__ __forceinline__ Sums operator+(const Sums& o) const {
+    return {query + o.query, context + o.context, pages + o.pages};
+  }
+};
+
+__device__ __forceinline__ Sums shuffle_up(const Sums& s, int by) {
+  return {__shfl_up_sync(0xffffffffu, s.query, by), __shfl_up_sync(0xffffffffu, s.context, by),
+          __shfl_up_sync(0xffffffffu, s.pages, by)};
+}
+
+__device__ __forceinline__ int32_t to_int32(int64_t x) { return int32_t(min(x, int64_t(0x7fffffff))); }
+
+// Position and slot of token i, which belongs to sequence b.
+__device__ __forceinline__ void place_token(const TableParams& p, int i, int b, const int32_t* first_token,
+                                            const int32_t* first_page, int64_t& pos, int32_t& slot) {
+  const unsigned c = cached(p, b), at = c + unsigned(i - first_token[b]);
+  const unsigned j = at / p.block_size, off = at - j * p.block_size;
+  pos = at;
+  slot = -1;
+  int64_t page = -1;
+  if (j < unsigned(p.max_blocks)) {
+    const unsigned have = pages_of(p, c);
+    if (j < have) {
+      page = p.block_tables[b * p.bt_stride + j];
+    } else {
+      const int64_t k = int64_t(first_page[b]) + j - have;
+      if (k < p.num_free) page = p.free_blocks[k];
     }
-    if (pages > p.num_free) s_err |= HL_TABLES_NO_PAGES;
-    if (q > p.max_tokens) s_err |= HL_TABLES_TOO_MANY_TOKENS;
-    p.status[0] = int32_t(pages < p.num_free ? pages : p.num_free);
-    p.status[1] = s_err;
+  }
+  const int64_t s = page * p.block_size + off;
+  if (page >= 0 && s <= 0x7fffffff) slot = int32_t(s);
+}
+
+__global__ void __launch_bounds__(kTableThreads) extend_tables_kernel(const TableParams p) {
+  extern __shared__ int32_t table_smem[];
+  int32_t* first_token = table_smem;                   // [num_seqs + 1]
+  int32_t* first_page = table_smem + p.num_seqs + 1;   // [num_seqs] index into free_blocks
+  __shared__ Sums warp_sums[kTableThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  // ---- prefix sums over the sequences
+  const int per = (p.num_seqs + kTableThreads - 1) / kTableThreads;
+  const int b0 = min(int(threadIdx.x) * per, p.num_seqs), b1 = min(b0 + per, p.num_seqs);
+  auto of = [&](int b) {
+    const unsigned c = cached(p, b), n = max(p.query_lens[b], 0);
+    return Sums{n, int64_t(c) + n, n ? pages_of(p, c + n) - pages_of(p, c) : 0};
+  };
+  Sums mine{0, 0, 0};
+  for (int b = b0; b < b1; ++b) mine = mine + of(b);
+  Sums upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const Sums v = shuffle_up(upto, o);
+    if (lane >= o) upto = upto + v;
+  }
+  if (lane == 31) warp_sums[warp] = upto;
+  __syncthreads();
+  Sums at{upto.query - mine.query, upto.context - mine.context, upto.pages - mine.pages}, total{0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kTableThreads / 32; ++w) {
+    if (w < warp) at = at + warp_sums[w];
+    total = total + warp_sums[w];
+  }
+  const bool writer = blockIdx.x == 0;
+  bool narrow = false;
+  for (int b = b0; b < b1; ++b) {
+    const Sums s = of(b);
+    first_token[b] = to_int32(at.query);
+    first_page[b] = to_int32(at.pages);
+    at = at + s;
+    if (writer) {
+      p.cu_seqlens_q[b + 1] = to_int32(at.query);
+      p.cu_seqlens_k[b + 1] = to_int32(at.context);
+      p.context_lens[b] = to_int32(s.context);
+      narrow |= s.query > 0 && s.context > int64_t(p.max_blocks) * p.block_size;
+    }
+  }
+  narrow = __syncthreads_or(narrow);
+  if (threadIdx.x == 0) {
+    first_token[p.num_seqs] = to_int32(total.query);
+    if (writer) {
+      p.cu_seqlens_q[0] = p.cu_seqlens_k[0] = 0;
+      p.status[0] = to_int32(min(total.pages, p.num_free));
+      p.status[1] = (total.pages > p.num_free ? HL_TABLES_NO_PAGES : 0) | (narrow ? HL_TABLES_TOO_NARROW : 0) |
+                    (total.query > p.max_tokens ? HL_TABLES_TOO_MANY_TOKENS : 0);
+    }
   }
   __syncthreads();
-  for (int b = threadIdx.x >> 5; b < p.num_seqs; b += kTableThreads / 32) {
-    const int64_t c = cached(p, b), n = max(p.query_lens[b], 0);
-    const int64_t have = pages_of(p, c), need = n > 0 ? pages_of(p, c + n) : have;
-    for (int64_t j = have + (threadIdx.x & 31); j < p.max_blocks; j += 32) {
-      const int64_t at = s_start[b] + j - have;
-      p.block_tables[b * p.bt_stride + j] = j < need && at < p.num_free ? p.free_blocks[at] : -1;
+
+  // ---- table rows, one warp each
+  for (int b = blockIdx.x * (kTableThreads / 32) + warp; b < p.num_seqs; b += gridDim.x * (kTableThreads / 32)) {
+    const unsigned c = cached(p, b), n = max(p.query_lens[b], 0);
+    const unsigned have = pages_of(p, c), need = n ? pages_of(p, c + n) : have;
+    for (unsigned j = have + lane; j < unsigned(p.max_blocks); j += 32) {
+      const int64_t k = int64_t(first_page[b]) + j - have;
+      p.block_tables[b * p.bt_stride + j] = j < need && k < p.num_free ? p.free_blocks[k] : -1;
     }
   }
-}
 
-// One thread per token: its sequence by binary search in cu_seqlens_q.
-__global__ void __launch_bounds__(256) token_slots_kernel(const TableParams p) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= p.max_tokens) return;
-  int lo = 0, hi = p.num_seqs;  // first sequence whose end lies behind i
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_seqlens_q[mid + 1] > i) hi = mid; else lo = mid + 1;
+  // ---- tokens, four neighbours a thread
+  const int64_t stride = int64_t(gridDim.x) * kTableThreads * kTokensPerThread;
+  for (int64_t i0 = (int64_t(blockIdx.x) * kTableThreads + threadIdx.x) * kTokensPerThread; i0 < p.max_tokens; i0 += stride) {
+    int lo = 0, hi = p.num_seqs;  // the sequence of token i0: the first that ends behind it
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (first_token[mid + 1] > i0) hi = mid; else lo = mid + 1;
+    }
+    int64_t pos[kTokensPerThread];
+    int32_t slot[kTokensPerThread];
+#pragma unroll
+    for (int k = 0; k < kTokensPerThread; ++k) {
+      const int64_t i = i0 + k;
+      while (lo < p.num_seqs && first_token[lo + 1] <= i) ++lo;
+      pos[k] = 0;
+      slot[k] = -1;
+      if (lo < p.num_seqs && i < p.max_tokens) place_token(p, int(i), lo, first_token, first_page, pos[k], slot[k]);
+    }
+    if (p.wide && i0 + kTokensPerThread <= p.max_tokens) {
+      *reinterpret_cast<longlong2*>(p.positions + i0) = make_longlong2(pos[0], pos[1]);
+      *reinterpret_cast<longlong2*>(p.positions + i0 + 2) = make_longlong2(pos[2], pos[3]);
+      *reinterpret_cast<int4*>(p.slot_mapping + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kTokensPerThread; ++k) {
+        if (i0 + k >= p.max_tokens) break;
+        p.positions[i0 + k] = pos[k];
+        p.slot_mapping[i0 + k] = slot[k];
+      }
+    }
   }
-  int64_t pos = 0;
-  int32_t slot = -1;
-  if (lo < p.num_seqs) {
-    pos = cached(p, lo) + i - p.cu_seqlens_q[lo];
-    const int64_t j = pos / p.block_size;
-    const int64_t page = j < p.max_blocks ? p.block_tables[lo * p.bt_stride + j] : -1;
-    const int64_t s = page * p.block_size + pos % p.block_size;
-    if (page >= 0 && s <= 0x7fffffff) slot = int32_t(s);
-  }
-  p.positions[i] = pos;
-  p.slot_mapping[i] = slot;
 }
 
 }  // namespace
@@ -128,13 +210,13 @@ extern "C" int hl_extend_block_tables(const int32_t* cached_lens, const int32_t*
                "hl_extend_block_tables: null pointer");
   const TableParams p{cached_lens, query_lens, num_seqs, block_tables, bt_stride, max_blocks, free_blocks, num_free,
                       block_size, max_tokens, cu_seqlens_q, cu_seqlens_k, context_lens, positions, slot_mapping,
-                      status};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  extend_tables_kernel<<<1, kTableThreads, 0, s>>>(p);
+                      status, aligned16(positions) && aligned16(slot_mapping)};
+  // One block per 1024 tokens or 8 table rows, whichever asks for more.
+  const int64_t by_tokens = (max_tokens + kTableThreads * kTokensPerThread - 1) / (kTableThreads * kTokensPerThread);
+  const int64_t by_rows = (num_seqs + kTableThreads / 32 - 1) / (kTableThreads / 32);
+  const int64_t want = by_tokens > by_rows ? by_tokens : by_rows;
+  const int blocks = want < 1 ? 1 : want > kMaxTableBlocks ? kMaxTableBlocks : int(want);
+  extend_tables_kernel<<<blocks, kTableThreads, (2 * num_seqs + 1) * sizeof(int32_t), static_cast<cudaStream_t>(stream)>>>(p);
   HL_CHECK_LAUNCH("hl_extend_block_tables");
-  if (max_tokens > 0) {
-    token_slots_kernel<<<unsigned((max_tokens + 255) / 256), 256, 0, s>>>(p);
-    HL_CHECK_LAUNCH("hl_extend_block_tables");
-  }
   return HL_OK;
 }

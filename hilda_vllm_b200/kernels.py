@@ -444,11 +444,12 @@ def _on_one_device(first: torch.Tensor, *rest: torch.Tensor) -> None:
 def _launch(name: str, t: torch.Tensor, *args) -> None:
     """Calls the C entry point `name` on t's device, current or not, and that device's stream."""
     fn = getattr(_lib.load(), name)
-    if t.get_device() == torch.cuda.current_device():
-        check(fn(*args, _stream(t)), name)
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)), name)
     else:
-        with torch.cuda.device(t.device):
-            check(fn(*args, _stream(t)), name)
+        with torch.cuda.device(dev):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)), name)
 
 
 def extend_block_tables(block_tables: torch.Tensor, cached_lens: torch.Tensor | None, query_lens: torch.Tensor,
@@ -472,12 +473,10 @@ def extend_block_tables(block_tables: torch.Tensor, cached_lens: torch.Tensor | 
         assert cached_lens.dtype == torch.int32 and cached_lens.is_contiguous() and cached_lens.shape == (b,)
     assert free_blocks.dtype == torch.int32 and free_blocks.is_contiguous() and free_blocks.dim() == 1
     dev = block_tables.device
-    cu_q = torch.empty(b + 1, dtype=torch.int32, device=dev)
-    cu_k = torch.empty(b + 1, dtype=torch.int32, device=dev)
-    context = torch.empty(b, dtype=torch.int32, device=dev)
+    # One allocation for the int32 results (slots first: 16-byte stores), one for the positions.
+    slots, cu_q, cu_k, context, status = torch.empty(max_tokens + 3 * b + 4, dtype=torch.int32, device=dev).split(
+        (max_tokens, b + 1, b + 1, b, 2))
     positions = torch.empty(max_tokens, dtype=torch.int64, device=dev)
-    slots = torch.empty(max_tokens, dtype=torch.int32, device=dev)
-    status = torch.empty(2, dtype=torch.int32, device=dev)
     _launch(
         "hl_extend_block_tables", block_tables, _p(cached_lens), query_lens.data_ptr(), b, block_tables.data_ptr(),
         block_tables.stride(0), width, free_blocks.data_ptr(), free_blocks.numel(), int(block_size), int(max_tokens),
