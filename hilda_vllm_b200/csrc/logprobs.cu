@@ -6,16 +6,73 @@
 // Sums are fp32.  A masked token (-inf) has probability 0 and adds nothing to the entropy; a row
 // with nothing but -inf has log probabilities -inf and entropy 0; a token id outside [0, vocab) has
 // log probability -inf; a NaN or +inf makes the row's results NaN, and a NaN ranks below -inf.
+//
+// Bound: one read of the logits from HBM.  A row is split over a cluster of thread blocks when there
+// are few rows (they meet in distributed shared memory), each thread keeps an online softmax of the
+// 16-byte vectors tid, tid + 512, ... of its block's piece: m, Z and S = sum 2^y y in units of
+// y = (x - m) log2 e, the exponential being the instruction that bounds it next (one per logit).
+// Alternatives come from the same pass.  The largest logit of each of 64 groups of threads is known;
+// the top_n-th largest of those is a threshold that at least top_n logits reach, and few more do
+// (some 24 for 20 of 151936 independent ones).  Only threads whose own maximum reaches it are looked
+// through again, a warp for one thread's vectors, and the candidates are ranked by unique 64-bit
+// (logit, index) keys.  Where ties at the threshold are too many for the candidate buffer, those with
+// the lowest indices are taken in index order; where that many lie above it, rounds of block maxima.
 #include "hl_common.cuh"
+
+#include <cooperative_groups.h>
 
 namespace hl {
 namespace {
 
-constexpr int kLpThreads = 1024;
+namespace cg = cooperative_groups;
+
+constexpr int kLpThreads = 512;
+constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kMaxTop = 32;
+constexpr int kGroups = 64;                     // threads tid = g mod 64, for the threshold
+constexpr int kMaxCandidates = 1024;
+constexpr int kMaxCluster = 8;
+constexpr int kUnroll = 4;                      // 16-byte loads in flight per thread
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <typename T>
+struct Row {
+  static constexpr int kVec = 16 / int(sizeof(T));
+  const T* x;        // the row
+  int head;          // logits in front of the first 16-byte boundary
+  int vectors;       // whole vectors behind it
+  int tail;          // logits behind those
+  __device__ __forceinline__ Row(const T* row, int vocab) : x(row) {
+    const int off = int(reinterpret_cast<uintptr_t>(row) & 15u) / int(sizeof(T));
+    head = min(off ? kVec - off : 0, vocab);
+    vectors = (vocab - head) / kVec;
+    tail = vocab - head - vectors * kVec;
+  }
+  __device__ __forceinline__ uint4 vector(int v) const { return __ldg(reinterpret_cast<const uint4*>(x + head) + v); }
+};
 
 __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float load_logit(const float* p) { return *p; }
+
+// Logits 2i and 2i + 1 of a vector.
+__device__ __forceinline__ float2 pair(const uint4& v, int i, const __nv_bfloat16*) {
+  const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+  return make_float2(bf16lo(w), bf16hi(w));
+}
+__device__ __forceinline__ float2 pair(const uint4& v, int i, const float*) {
+  return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
+                : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+}
+// Largest logit of a vector (NaN ignored).
+__device__ __forceinline__ float vector_max(const uint4& v, const __nv_bfloat16*) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float vector_max(const uint4& v, const float*) {
+  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
 
 // Whole numbers in the order of the logits: NaN lowest, then -inf ... +inf; -0 and +0 alike.  Never 0.
 __device__ __forceinline__ uint32_t logit_key(float x) {
@@ -23,91 +80,395 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-
-// Unique over a row: larger for a larger logit, and for a lower index among equals.
-__device__ __forceinline__ uint64_t entry_key(float x, int i) {
-  return (uint64_t(logit_key(x)) << 32) | uint32_t(~i);
+__device__ __forceinline__ float key_logit(uint32_t k) {
+  if (k == 1u) return NAN;
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 
+// Unique over a row: larger for a larger logit, and for a lower index among equals.  Never 0.
+__device__ __forceinline__ uint64_t entry_key(uint32_t key, int i) { return (uint64_t(key) << 32) | uint32_t(~i); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Keeps NaN (fmaxf would not); -inf becomes -1000, whose power of two is 0 and stays 0 when multiplied.
+__device__ __forceinline__ float floor_exponent(float y) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0fC47A0000;" : "=f"(r) : "f"(y));
+  return r;
+}
+
+// Online softmax: z = sum 2^y, s = sum 2^y y, y = (x - m) log2 e.
+struct Softmax {
+  float m, z, s;
+
+  __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }
+  __device__ __forceinline__ void raise(float to) {
+    if (!(to > m)) return;
+    if (m != -INFINITY) {
+      const float d = floor_exponent((m - to) * kLog2e), f = ex2(d);
+      s = f * fmaf(d, z, s);
+      z *= f;
+    }
+    m = to;
+  }
+  __device__ __forceinline__ void add(float x) {
+    raise(x);
+    const float y = floor_exponent((x - ref()) * kLog2e), e = ex2(y);
+    z += e;
+    s = fmaf(e, y, s);
+  }
+  // Another part's sums; the maximum is the larger of both.
+  __device__ __forceinline__ void merge(const Softmax& o) {
+    raise(o.m);
+    if (o.m == -INFINITY) {  // nothing but -inf, or NaN
+      z += o.z;
+      s += o.s;
+      return;
+    }
+    const float d = floor_exponent((o.m - ref()) * kLog2e), f = ex2(d);
+    z = fmaf(o.z, f, z);
+    s += f * fmaf(d, o.z, o.s);
+  }
+};
+
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+struct LpShared {
+  Softmax parts[kLpWarps];
+  Softmax sum;
+  uint32_t group_key[kGroups];
+  uint32_t threshold;
+  int count;                      // of candidates
+  int scan[kLpWarps];
+  uint64_t best;
+  uint64_t candidates[kMaxCandidates];
+  uint64_t top[kMaxTop];          // this block's, in order; 0 behind the last
+  uint64_t all[kMaxCluster * kMaxTop];
+};
+
+// This block's piece of a row.
 template <typename T>
-__device__ T block_max(T v, T* shared) {
+struct Piece {
+  Row<T> row;
+  int begin, end;      // vectors
+  bool first, last;    // has the head, the tail
+  // Calls f(logit, index) for every logit of thread `t`, vectors first.
+  template <typename F>
+  __device__ __forceinline__ void each_of(int t, F f) const {
+    for (int v = begin + t; v < end; v += kLpThreads) each_in(v, f);
+    each_single(t, f);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each_in(int v, F f) const {
+    const uint4 q = row.vector(v);
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    const T w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
+    for (int i = 0; i < Row<T>::kVec / 2; ++i) {
+      const float2 x = pair(q, i, row.x);
+      f(x.x, row.head + v * Row<T>::kVec + 2 * i);
+      f(x.y, row.head + v * Row<T>::kVec + 2 * i + 1);
+    }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each_single(int t, F f) const {
+    if (first && t < row.head) f(load_logit(row.x + t), t);
+    if (last && t < row.tail) {
+      const int i = row.head + row.vectors * Row<T>::kVec + t;
+      f(load_logit(row.x + i), i);
+    }
+  }
+};
+
+// The top_n largest entries of the piece, in order, into sh.top.  mine: the key of this thread's
+// largest logit, 0 if it has none.
+template <typename T>
+__device__ void block_top(const Piece<T>& piece, int top_n, uint32_t mine, LpShared& sh) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < kGroups) sh.group_key[tid] = 0;
+  if (tid < kMaxTop) sh.top[tid] = 0;
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  atomicMax(&sh.group_key[tid % kGroups], mine);
+  __syncthreads();
+  if (tid < kGroups) {
+    const uint32_t g = sh.group_key[tid];
+    int rank = 0;
+#pragma unroll 16
+    for (int i = 0; i < kGroups; ++i) {
+      const uint32_t o = sh.group_key[i];
+      rank += o > g || (o == g && i < tid);
+    }
+    if (rank == top_n - 1) sh.threshold = g;
   }
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  const uint32_t threshold = sh.threshold;
+  auto collect = [&](float x, int i, uint32_t least) {
+    const uint32_t key = logit_key(x);
+    if (key < least) return;
+    const int at = atomicAdd(&sh.count, 1);
+    if (at < kMaxCandidates) sh.candidates[at] = entry_key(key, i);
+  };
+  // Warps look through the vectors of their threads that reach `least`, one thread's at a time.
+  auto gather = [&](uint32_t least) {
+    for (unsigned todo = __ballot_sync(0xffffffffu, mine >= least); todo; todo &= todo - 1) {
+      const int t = warp * 32 + __ffs(todo) - 1;
+      for (int v = piece.begin + t + lane * kLpThreads; v < piece.end; v += 32 * kLpThreads)
+        piece.each_in(v, [&](float x, int i) { collect(x, i, least); });
+    }
+    if (mine >= least) piece.each_single(tid, [&](float x, int i) { collect(x, i, least); });
+  };
+  gather(threshold);
   __syncthreads();
-  v = shared[0];
-  for (int w = 1; w < kLpThreads / 32; ++w) v = shared[w] > v ? shared[w] : v;
-  return v;
-}
-
-__device__ float block_sum(float v, float* shared) {
+  int count = sh.count;
+  if (count > kMaxCandidates) {
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    gather(threshold + 1);
+    __syncthreads();
+    count = sh.count;
+    if (count <= kMaxCandidates) {
+      // The ties at the threshold with the lowest indices: head, then vectors, then tail.
+      int need = top_n - count;
+      auto take = [&](int ties, auto each) {  // ties of this thread, in index order over the threads
+        int upto = ties;
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        __syncthreads();
+        if (lane == 31) sh.scan[warp] = upto;
+        __syncthreads();
+        int before = upto - ties, total = 0;
+        for (int w = 0; w < kLpWarps; ++w) {
+          if (w < warp) before += sh.scan[w];
+          total += sh.scan[w];
+        }
+        int at = before;
+        each([&](int i) {
+          if (at < need) sh.candidates[count + at] = entry_key(threshold, i);
+          ++at;
+        });
+        const int took = min(total, need);
+        need -= took;
+        count += took;
+      };
+      auto tied = [&](float x) { return logit_key(x) == threshold; };
+      auto single = [&](bool has, int i) {
+        const bool t = has && tied(load_logit(piece.row.x + i));
+        take(t, [&](auto put) { if (t) put(i); });
+      };
+      if (need > 0 && piece.first) single(tid < piece.row.head, tid);
+      for (int v = piece.begin; need > 0 && v < piece.end; v += kLpThreads) {
+        int ties = 0;
+        if (v + tid < piece.end) piece.each_in(v + tid, [&](float x, int) { ties += tied(x); });
+        take(ties, [&](auto put) {
+          if (ties) piece.each_in(v + tid, [&](float x, int i) { if (tied(x)) put(i); });
+        });
+      }
+      if (need > 0 && piece.last) single(tid < piece.row.tail, piece.row.head + piece.row.vectors * Row<T>::kVec + tid);
+      __syncthreads();
+    } else {
+      // More above the threshold than the buffer holds: one block maximum per alternative.
+      uint64_t below = ~0ull;
+      for (int r = 0; r < top_n; ++r) {
+        uint64_t best = 0;
+        if (mine >= threshold)
+          piece.each_of(tid, [&](float x, int i) {
+            const uint64_t e = entry_key(logit_key(x), i);
+            if (e < below && e > best) best = e;
+          });
+        __syncthreads();
+        if (tid == 0) sh.best = 0;
+        __syncthreads();
+        if (best) atomicMax(reinterpret_cast<unsigned long long*>(&sh.best), best);
+        __syncthreads();
+        below = sh.best;
+        if (tid == 0) sh.top[r] = below;
+      }
+      __syncthreads();
+      return;
+    }
+  }
+  for (int i = tid; i < count; i += kLpThreads) {
+    const uint64_t e = sh.candidates[i];
+    int rank = 0;
+    for (int j = 0; j < count; ++j) rank += sh.candidates[j] > e;
+    if (rank < top_n) sh.top[rank] = e;
+  }
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < kLpThreads / 32; ++w) v += shared[w];
-  return v;
 }
 
-// One thread block per row, three passes and one more per alternative.
+// One cluster per row, each block a piece of it.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(
+__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, const int64_t* __restrict__ tokens, int top_n,
     float* __restrict__ logprobs, float* __restrict__ entropies, int64_t* __restrict__ top_tokens,
     float* __restrict__ top_logprobs) {
-  __shared__ uint64_t s64[32];
-  __shared__ float sf[32];
-  const int64_t row = blockIdx.x;
-  const T* x = logits + row * row_stride;
-  uint64_t best = 0;
-  float nan = 0.f;
-  for (int i = threadIdx.x; i < vocab; i += kLpThreads) {
-    const float v = load_logit(x + i);
-    const uint64_t k = entry_key(v, i);
-    best = k > best ? k : best;
-    if (v != v) nan = v;
-  }
-  best = block_max(best, s64);
-  const float m = load_logit(x + int(~uint32_t(best)));
-  float z = nan, s = 0.f;
-  for (int i = threadIdx.x; i < vocab; i += kLpThreads) {
-    const float v = load_logit(x + i);
-    if (v == -INFINITY) continue;
-    const float e = expf(v - m);
-    z += e;
-    s += e * (v - m);
-  }
-  z = block_sum(z, sf);
-  s = block_sum(s, sf);
-  const float log_z = z != z ? z : (m == -INFINITY ? INFINITY : logf(z));
-  if (threadIdx.x == 0) {
-    const int64_t t = tokens[row];
-    const float xt = t >= 0 && t < vocab ? load_logit(x + t) : -INFINITY;
-    logprobs[row] = (xt == -INFINITY && log_z == log_z) ? -INFINITY : xt - m - log_z;
-    entropies[row] = m == -INFINITY && z == z ? 0.f : log_z - s / z;
-  }
-  for (int r = 0; r < top_n; ++r) {
-    if (r > 0) {
-      uint64_t next = 0;
-      for (int i = threadIdx.x; i < vocab; i += kLpThreads) {
-        const uint64_t k = entry_key(load_logit(x + i), i);
-        if (k < best && k > next) next = k;
+  __shared__ LpShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  const int64_t row_at = blockIdx.x / blocks;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Row<T> row(logits + row_at * row_stride, vocab);
+  const Piece<T> piece{row, int(int64_t(row.vectors) * rank / blocks), int(int64_t(row.vectors) * (rank + 1) / blocks),
+                       rank == 0, rank == blocks - 1};
+  Softmax sm{-INFINITY, 0.f, 0.f};
+  float thread_max = NAN;  // NaN: nothing else
+  bool any = false;        // the thread has a logit
+  piece.each_single(tid, [&](float x, int) {
+    sm.add(x);
+    thread_max = fmaxf(thread_max, x);
+    any = true;
+  });
+  any |= piece.begin + tid < piece.end;
+  for (int v0 = piece.begin + tid; v0 < piece.end; v0 += kUnroll * kLpThreads) {
+    uint4 q[kUnroll];
+    if (v0 + (kUnroll - 1) * kLpThreads < piece.end) {
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) q[k] = row.vector(v0 + k * kLpThreads);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        // Behind the piece: NaN for the maximum, replaced by -inf, which adds nothing, below.
+        q[k] = v0 + k * kLpThreads < piece.end ? row.vector(v0 + k * kLpThreads) : make_uint4(~0u, ~0u, ~0u, ~0u);
       }
-      best = block_max(next, s64);
     }
-    if (threadIdx.x == 0) {
-      const int i = int(~uint32_t(best));
-      const float v = load_logit(x + i);
-      top_tokens[row * top_n + r] = i;
-      top_logprobs[row * top_n + r] = (v == -INFINITY && log_z == log_z) ? -INFINITY : v - m - log_z;
+    float mx = vector_max(q[0], row.x);
+#pragma unroll
+    for (int k = 1; k < kUnroll; ++k) mx = fmaxf(mx, vector_max(q[k], row.x));
+    thread_max = fmaxf(thread_max, mx);
+    if (v0 + (kUnroll - 1) * kLpThreads >= piece.end) {
+      const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+#pragma unroll
+      for (int k = 1; k < kUnroll; ++k)
+        if (v0 + k * kLpThreads >= piece.end) q[k] = make_uint4(none, none, none, none);
+    }
+    sm.raise(mx);
+    const float minus = -sm.ref();
+    const uint64_t off = f32x2(minus, minus), scale = f32x2(kLog2e, kLog2e);
+    uint64_t z = 0, s = 0;  // (0.f, 0.f)
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+#pragma unroll
+      for (int i = 0; i < Row<T>::kVec / 2; ++i) {
+        const float2 x = pair(q[k], i, row.x);
+        const float2 y = unpack(mul2(add2(f32x2(x.x, x.y), off), scale));
+        const float y0 = floor_exponent(y.x), y1 = floor_exponent(y.y);
+        const uint64_t e = f32x2(ex2(y0), ex2(y1));
+        z = add2(z, e);
+        s = fma2(e, f32x2(y0, y1), s);
+      }
+    }
+    const float2 zz = unpack(z), ss = unpack(s);
+    sm.z += zz.x + zz.y;
+    sm.s += ss.x + ss.y;
+  }
+  // ---- the block's sums
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    Softmax other;
+    other.m = __shfl_xor_sync(0xffffffffu, sm.m, o);
+    other.z = __shfl_xor_sync(0xffffffffu, sm.z, o);
+    other.s = __shfl_xor_sync(0xffffffffu, sm.s, o);
+    sm.merge(other);
+  }
+  if (lane == 0) sh.parts[warp] = sm;
+  if (top_n > 0) block_top(piece, top_n, any ? logit_key(thread_max) : 0u, sh);
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kLpWarps; ++w) sm.merge(sh.parts[w]);
+    sh.sum = sm;
+  }
+  if (blocks > 1) {
+    cluster.sync();
+    if (rank == 0) {
+      if (tid == 0)
+        for (int b = 1; b < blocks; ++b) sm.merge(*cluster.map_shared_rank(&sh.sum, b));
+      const int n = blocks * top_n;
+      if (tid < n) sh.all[tid] = cluster.map_shared_rank(sh.top, tid / top_n)[tid % top_n];
+    }
+    cluster.sync();  // the others' shared memory has been read
+    if (rank != 0) return;
+    if (tid == 0) sh.sum = sm;
+    if (tid < kMaxTop) sh.top[tid] = 0;
+    __syncthreads();
+    const int n = blocks * top_n;
+    if (tid < n && sh.all[tid] != 0) {
+      const uint64_t e = sh.all[tid];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += sh.all[j] > e;
+      if (r < top_n) sh.top[r] = e;
     }
   }
+  __syncthreads();
+  // ---- results
+  const Softmax sum = sh.sum;
+  const float log_z = sum.z != sum.z ? sum.z : log2f(sum.z);
+  const bool masked = sum.m == -INFINITY && sum.z == sum.z;  // every logit is -inf
+  auto logprob = [&](float x) {
+    if (x == -INFINITY && sum.z == sum.z) return -INFINITY;
+    return ((x - sum.m) * kLog2e - log_z) * kLn2;
+  };
+  if (tid == 0) {
+    const int64_t t = tokens[row_at];
+    logprobs[row_at] = logprob(t >= 0 && t < vocab ? load_logit(row.x + t) : -INFINITY);
+    entropies[row_at] = masked ? 0.f : (log_z - sum.s / sum.z) * kLn2;
+  }
+  if (tid < top_n) {
+    const uint64_t e = sh.top[tid];
+    top_tokens[row_at * top_n + tid] = int(~uint32_t(e));
+    top_logprobs[row_at * top_n + tid] = logprob(key_logit(uint32_t(e >> 32)));
+  }
+}
+
+template <typename T>
+cudaError_t launch_logprobs(const void* logits, int64_t row_stride, int64_t rows, int vocab, const int64_t* tokens, int top_n,
+                            float* logprobs, float* entropies, int64_t* top_tokens, float* top_logprobs, cudaStream_t stream) {
+  // Blocks per row: enough that three blocks an SM are busy, as long as a thread keeps a full batch of loads.
+  int blocks = 1;
+  while (blocks < kMaxCluster && rows * blocks < 3 * 148 &&
+         vocab / (2 * blocks) >= kLpThreads * kUnroll * Row<T>::kVec / 2)
+    blocks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(rows * blocks));
+  cfg.blockDim = dim3(kLpThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, static_cast<const T*>(logits), row_stride, vocab, tokens,
+                            top_n, logprobs, entropies, top_tokens, top_logprobs);
 }
 
 }  // namespace
@@ -127,14 +488,14 @@ extern "C" int hl_token_logprobs(const void* logits, int logits_fp32, int64_t ro
   HL_CHECK_ARG(logits && token_ids && logprobs && entropies && (top_n == 0 || (top_tokens && top_logprobs)),
                "hl_token_logprobs: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (logits_fp32) {
-    token_logprobs_kernel<float><<<unsigned(rows), kLpThreads, 0, s>>>(
-        static_cast<const float*>(logits), row_stride, vocab, token_ids, top_n, logprobs, entropies, top_tokens,
-        top_logprobs);
-  } else {
-    token_logprobs_kernel<__nv_bfloat16><<<unsigned(rows), kLpThreads, 0, s>>>(
-        static_cast<const __nv_bfloat16*>(logits), row_stride, vocab, token_ids, top_n, logprobs, entropies,
-        top_tokens, top_logprobs);
+  const cudaError_t e =
+      logits_fp32 ? launch_logprobs<float>(logits, row_stride, rows, vocab, token_ids, top_n, logprobs, entropies,
+                                           top_tokens, top_logprobs, s)
+                  : launch_logprobs<__nv_bfloat16>(logits, row_stride, rows, vocab, token_ids, top_n, logprobs,
+                                                   entropies, top_tokens, top_logprobs, s);
+  if (e != cudaSuccess) {
+    set_error("hl_token_logprobs: launch failed: %s", cudaGetErrorString(e));
+    return HL_ERR_CUDA;
   }
   HL_CHECK_LAUNCH("hl_token_logprobs");
   return HL_OK;

@@ -523,6 +523,35 @@ def test_logprobs_rows_without_a_finite_value(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logprobs_crowded_top(dtype):
+    """Thousands of logits above what the rest of the row reaches, in a few columns of the 16-byte
+    vectors; and thousands of ties at the last alternative, some in front of the larger logits."""
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn(4, 151936, generator=g, device=DEV)
+    column = torch.arange(151936, device=DEV) % 4096
+    x[0, column < 64] += 100
+    x[1, column < 32] += 100
+    x[2] = torch.where(column < 2000, 7.0, x[2])
+    x[2, 5000:5010] = torch.arange(8.0, 18.0, device=DEV)
+    x[3, 100000:] = 3.0
+    x[3, :100000].clamp_(max=2.0)
+    for top in (2, 20, 32):
+        check_logprobs(x.to(dtype), torch.tensor([3, 1, 2, 150000], device=DEV), top)
+        check_logprobs(x.to(dtype).repeat(200, 1)[:, 1:], torch.randint(0, 151935, (800,), generator=g, device=DEV), top)
+
+
+@pytest.mark.parametrize("vocab,nans", [(5, 3), (40, 20), (300, 299), (20011, 20000), (9000, 9000)])
+def test_logprobs_nan_ranks_last(vocab, nans):
+    g = torch.Generator(device=DEV).manual_seed(12)
+    x = torch.randn(3, vocab, generator=g, device=DEV)
+    x[:, torch.randperm(vocab, generator=g, device=DEV)[:nans]] = math.nan
+    top = min(vocab, 32)
+    _, _, ids, _ = kernels.token_logprobs(x, torch.zeros(3, dtype=torch.int64, device=DEV), top)
+    key = torch.where(x.isnan(), -math.inf, x)
+    assert torch.equal(ids, torch.sort(key, dim=-1, descending=True, stable=True).indices[:, :top])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_logprobs_strided_and_unaligned_rows(dtype):
     g = torch.Generator(device=DEV).manual_seed(10)
     wide = (torch.randn(9, 5003, generator=g, device=DEV) * 3).to(dtype)
