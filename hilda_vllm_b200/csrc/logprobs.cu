@@ -9,8 +9,10 @@
 //
 // Bound: one read of the logits from HBM.  A row is split over a cluster of thread blocks when there
 // are few rows (they meet in distributed shared memory), each thread keeps an online softmax of the
-// 16-byte vectors tid, tid + 512, ... of its block's piece: m, Z and S = sum 2^y y in units of
-// y = (x - m) log2 e, the exponential being the instruction that bounds it next (one per logit).
+// 16-byte vectors tid, tid + T, ... of its block's piece (T threads): Z = sum 2^y and S = sum 2^y y, where
+// y = x log2 e - R and R a whole number near its maximum, raised only when a logit exceeds it by far
+// (2^16): one FMA a logit, and parts of different R meet with exact powers of two.  The exponential
+// (one MUFU a logit) bounds it next.
 // Alternatives come from the same pass.  The largest logit of each of 64 groups of threads is known;
 // the top_n-th largest of those is a threshold that at least top_n logits reach, and few more do
 // (some 24 for 20 of 151936 independent ones).  Only threads whose own maximum reaches it are looked
@@ -26,8 +28,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpThreads = 512;
-constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kGroups = 64;                     // threads tid = g mod 64, for the threshold
 constexpr int kMaxCandidates = 1024;
@@ -64,14 +64,22 @@ __device__ __forceinline__ float2 pair(const uint4& v, int i, const float*) {
   return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
                 : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
 }
-// Largest logit of a vector (NaN ignored).
-__device__ __forceinline__ float vector_max(const uint4& v, const __nv_bfloat16*) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  return fmaxf(__low2float(m), __high2float(m));
+// Largest and smallest logit of a batch of vectors (NaN ignored; NaN if there is nothing else).
+template <int N>
+__device__ __forceinline__ float2 extremes(const uint4 (&v)[N], const __nv_bfloat16*) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v[0]);
+  __nv_bfloat162 hi = h[0], lo = h[0];
+#pragma unroll
+  for (int i = 1; i < 4 * N; ++i) hi = __hmax2(hi, h[i]), lo = __hmin2(lo, h[i]);
+  return make_float2(fmaxf(__low2float(hi), __high2float(hi)), fminf(__low2float(lo), __high2float(lo)));
 }
-__device__ __forceinline__ float vector_max(const uint4& v, const float*) {
-  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+template <int N>
+__device__ __forceinline__ float2 extremes(const uint4 (&v)[N], const float*) {
+  const float* f = reinterpret_cast<const float*>(&v[0]);
+  float hi = f[0], lo = f[0];
+#pragma unroll
+  for (int i = 1; i < 4 * N; ++i) hi = fmaxf(hi, f[i]), lo = fminf(lo, f[i]);
+  return make_float2(hi, lo);
 }
 
 // Whole numbers in the order of the logits: NaN lowest, then -inf ... +inf; -0 and +0 alike.  Never 0.
@@ -100,39 +108,57 @@ __device__ __forceinline__ float floor_exponent(float y) {
   return r;
 }
 
-// Online softmax: z = sum 2^y, s = sum 2^y y, y = (x - m) log2 e.
+// Logits from here on differ by more than any softmax resolves unless they are equal; log2 e times
+// them may overflow.
+constexpr float kHuge = 1e30f;
+
+// y of a logit x for a part with reference m, one of its logits and no less than its maximum - 11:
+// x log2 e - ceil(m log2 e), or (x - m) log2 e for a huge m; -1000 at least.
+__device__ __forceinline__ float origin(float m) { return ceilf(m * kLog2e); }
+__device__ __forceinline__ float exponent(float x, float m) {
+  return floor_exponent(fabsf(m) < kHuge ? fmaf(x, kLog2e, -origin(m)) : (x - m) * kLog2e);
+}
+
+// Online softmax: z = sum 2^y, s = sum 2^y y.
 struct Softmax {
   float m, z, s;
 
   __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }
   __device__ __forceinline__ void raise(float to) {
     if (!(to > m)) return;
-    if (m != -INFINITY) {
-      const float d = floor_exponent((m - to) * kLog2e), f = ex2(d);
+    if (m != -INFINITY) {  // else z and s are 0, or NaN
+      const float d = fabsf(m) < kHuge && fabsf(to) < kHuge ? floor_exponent(origin(m) - origin(to))
+                                                            : floor_exponent((m - to) * kLog2e);
+      const float f = ex2(d);
       s = f * fmaf(d, z, s);
       z *= f;
     }
     m = to;
   }
+  // The same where the reference would fall behind by more than 16 = 11 log2 e.
+  __device__ __forceinline__ void raise_late(float to) {
+    if (!(to <= m + 11.f)) raise(to);
+  }
   __device__ __forceinline__ void add(float x) {
-    raise(x);
-    const float y = floor_exponent((x - ref()) * kLog2e), e = ex2(y);
+    raise_late(x);
+    const float y = exponent(x, ref()), e = ex2(y);
     z += e;
     s = fmaf(e, y, s);
   }
-  // Another part's sums; the maximum is the larger of both.
-  __device__ __forceinline__ void merge(const Softmax& o) {
-    raise(o.m);
-    if (o.m == -INFINITY) {  // nothing but -inf, or NaN
-      z += o.z;
-      s += o.s;
-      return;
-    }
-    const float d = floor_exponent((o.m - ref()) * kLog2e), f = ex2(d);
-    z = fmaf(o.z, f, z);
-    s += f * fmaf(d, o.z, o.s);
-  }
 };
+
+// The sums of a warp's lanes (`lanes` of them, a power of two), in every one of those lanes.
+__device__ __forceinline__ Softmax warp_merge(Softmax a, int lanes) {
+  float m = a.m;
+  for (int o = lanes / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  a.raise(m);
+  for (int o = lanes / 2; o >= 1; o >>= 1) {
+    a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+  }
+  a.m = m;
+  return a;
+}
 
 __device__ __forceinline__ uint64_t f32x2(float a, float b) {
   uint64_t r;
@@ -149,24 +175,21 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 
+template <int NT>
 struct LpShared {
-  Softmax parts[kLpWarps];
+  Softmax parts[(NT / 32)];
   Softmax sum;
   uint32_t group_key[kGroups];
   uint32_t threshold;
-  int count;                      // of candidates
-  int scan[kLpWarps];
+  int count, suspects;            // candidates; threads whose maximum reaches the threshold
+  uint16_t suspect[NT];
+  int scan[(NT / 32)];
   uint64_t best;
   uint64_t candidates[kMaxCandidates];
   uint64_t top[kMaxTop];          // this block's, in order; 0 behind the last
@@ -174,7 +197,7 @@ struct LpShared {
 };
 
 // This block's piece of a row.
-template <typename T>
+template <typename T, int NT>
 struct Piece {
   Row<T> row;
   int begin, end;      // vectors
@@ -182,7 +205,7 @@ struct Piece {
   // Calls f(logit, index) for every logit of thread `t`, vectors first.
   template <typename F>
   __device__ __forceinline__ void each_of(int t, F f) const {
-    for (int v = begin + t; v < end; v += kLpThreads) each_in(v, f);
+    for (int v = begin + t; v < end; v += NT) each_in(v, f);
     each_single(t, f);
   }
   template <typename F>
@@ -207,12 +230,12 @@ struct Piece {
 
 // The top_n largest entries of the piece, in order, into sh.top.  mine: the key of this thread's
 // largest logit, 0 if it has none.
-template <typename T>
-__device__ void block_top(const Piece<T>& piece, int top_n, uint32_t mine, LpShared& sh) {
+template <typename T, int NT>
+__device__ void block_top(const Piece<T, NT>& piece, int top_n, uint32_t mine, LpShared<NT>& sh) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < kGroups) sh.group_key[tid] = 0;
   if (tid < kMaxTop) sh.top[tid] = 0;
-  if (tid == 0) sh.count = 0;
+  if (tid == 0) sh.count = sh.suspects = 0;
   __syncthreads();
   atomicMax(&sh.group_key[tid % kGroups], mine);
   __syncthreads();
@@ -234,21 +257,25 @@ __device__ void block_top(const Piece<T>& piece, int top_n, uint32_t mine, LpSha
     const int at = atomicAdd(&sh.count, 1);
     if (at < kMaxCandidates) sh.candidates[at] = entry_key(key, i);
   };
-  // Warps look through the vectors of their threads that reach `least`, one thread's at a time.
+  // The vectors of the threads whose maximum reaches `least`, spread over all threads.
   auto gather = [&](uint32_t least) {
-    for (unsigned todo = __ballot_sync(0xffffffffu, mine >= least); todo; todo &= todo - 1) {
-      const int t = warp * 32 + __ffs(todo) - 1;
-      for (int v = piece.begin + t + lane * kLpThreads; v < piece.end; v += 32 * kLpThreads)
-        piece.each_in(v, [&](float x, int i) { collect(x, i, least); });
+    if (mine >= least) {
+      sh.suspect[atomicAdd(&sh.suspects, 1)] = uint16_t(tid);
+      piece.each_single(tid, [&](float x, int i) { collect(x, i, least); });
     }
-    if (mine >= least) piece.each_single(tid, [&](float x, int i) { collect(x, i, least); });
+    __syncthreads();
+    const int each = (piece.end - piece.begin + NT - 1) / NT, n = sh.suspects * each;
+    for (int u = tid; u < n; u += NT) {
+      const int v = piece.begin + sh.suspect[u / each] + u % each * NT;
+      if (v < piece.end) piece.each_in(v, [&](float x, int i) { collect(x, i, least); });
+    }
   };
   gather(threshold);
   __syncthreads();
   int count = sh.count;
   if (count > kMaxCandidates) {
     __syncthreads();
-    if (tid == 0) sh.count = 0;
+    if (tid == 0) sh.count = sh.suspects = 0;
     __syncthreads();
     gather(threshold + 1);
     __syncthreads();
@@ -267,7 +294,7 @@ __device__ void block_top(const Piece<T>& piece, int top_n, uint32_t mine, LpSha
         if (lane == 31) sh.scan[warp] = upto;
         __syncthreads();
         int before = upto - ties, total = 0;
-        for (int w = 0; w < kLpWarps; ++w) {
+        for (int w = 0; w < (NT / 32); ++w) {
           if (w < warp) before += sh.scan[w];
           total += sh.scan[w];
         }
@@ -286,7 +313,7 @@ __device__ void block_top(const Piece<T>& piece, int top_n, uint32_t mine, LpSha
         take(t, [&](auto put) { if (t) put(i); });
       };
       if (need > 0 && piece.first) single(tid < piece.row.head, tid);
-      for (int v = piece.begin; need > 0 && v < piece.end; v += kLpThreads) {
+      for (int v = piece.begin; need > 0 && v < piece.end; v += NT) {
         int ties = 0;
         if (v + tid < piece.end) piece.each_in(v + tid, [&](float x, int) { ties += tied(x); });
         take(ties, [&](auto put) {
@@ -317,7 +344,7 @@ __device__ void block_top(const Piece<T>& piece, int top_n, uint32_t mine, LpSha
       return;
     }
   }
-  for (int i = tid; i < count; i += kLpThreads) {
+  for (int i = tid; i < count; i += NT) {
     const uint64_t e = sh.candidates[i];
     int rank = 0;
     for (int j = 0; j < count; ++j) rank += sh.candidates[j] > e;
@@ -327,19 +354,24 @@ __device__ void block_top(const Piece<T>& piece, int top_n, uint32_t mine, LpSha
 }
 
 // One cluster per row, each block a piece of it.
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, const int64_t* __restrict__ tokens, int top_n,
     float* __restrict__ logprobs, float* __restrict__ entropies, int64_t* __restrict__ top_tokens,
     float* __restrict__ top_logprobs) {
-  __shared__ LpShared sh;
+  __shared__ LpShared<NT> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   const int64_t row_at = blockIdx.x / blocks;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Row<T> row(logits + row_at * row_stride, vocab);
-  const Piece<T> piece{row, int(int64_t(row.vectors) * rank / blocks), int(int64_t(row.vectors) * (rank + 1) / blocks),
+  const Piece<T, NT> piece{row, int(int64_t(row.vectors) * rank / blocks), int(int64_t(row.vectors) * (rank + 1) / blocks),
                        rank == 0, rank == blocks - 1};
+  float asked = -INFINITY;  // the logit of the row's token
+  if (rank == 0 && tid == 0) {
+    const int64_t t = tokens[row_at];
+    if (t >= 0 && t < vocab) asked = load_logit(row.x + t);
+  }
   Softmax sm{-INFINITY, 0.f, 0.f};
   float thread_max = NAN;  // NaN: nothing else
   bool any = false;        // the thread has a logit
@@ -349,30 +381,36 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(
     any = true;
   });
   any |= piece.begin + tid < piece.end;
-  for (int v0 = piece.begin + tid; v0 < piece.end; v0 += kUnroll * kLpThreads) {
-    uint4 q[kUnroll];
-    if (v0 + (kUnroll - 1) * kLpThreads < piece.end) {
+  // Batches of kUnroll vectors, the next one's loads in flight while one is summed.
+  auto load = [&](uint4 (&q)[kUnroll], int v0) {
+    if (v0 + (kUnroll - 1) * NT < piece.end) {
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) q[k] = row.vector(v0 + k * kLpThreads);
+      for (int k = 0; k < kUnroll; ++k) q[k] = row.vector(v0 + k * NT);
     } else {
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) {
-        // Behind the piece: NaN for the maximum, replaced by -inf, which adds nothing, below.
-        q[k] = v0 + k * kLpThreads < piece.end ? row.vector(v0 + k * kLpThreads) : make_uint4(~0u, ~0u, ~0u, ~0u);
-      }
+      for (int k = 0; k < kUnroll; ++k)  // behind the piece: NaN, which no maximum takes
+        q[k] = v0 + k * NT < piece.end ? row.vector(v0 + k * NT) : make_uint4(~0u, ~0u, ~0u, ~0u);
     }
-    float mx = vector_max(q[0], row.x);
-#pragma unroll
-    for (int k = 1; k < kUnroll; ++k) mx = fmaxf(mx, vector_max(q[k], row.x));
-    thread_max = fmaxf(thread_max, mx);
-    if (v0 + (kUnroll - 1) * kLpThreads >= piece.end) {
-      const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+  };
+  auto sum_batch = [&](uint4 (&q)[kUnroll], int v0) {
+    if (v0 >= piece.end) return;
+    const float2 range = extremes(q, row.x);
+    thread_max = fmaxf(thread_max, range.x);
+    sm.raise_late(range.x);
+    if (!(range.y > -kHuge && sm.m < kHuge)) {  // masked or huge logits, or nothing but NaN: one by one
+      for (int k = 0; k < kUnroll; ++k) {
+        const int v = v0 + k * NT;
+        if (v < piece.end) piece.each_in(v, [&](float x, int) { sm.add(x); });
+      }
+      return;
+    }
+    if (v0 + (kUnroll - 1) * NT >= piece.end) {  // behind the piece: -9e29, which adds nothing
+      const uint32_t low = sizeof(T) == 2 ? 0xf135f135u : 0xf135be37u;
 #pragma unroll
       for (int k = 1; k < kUnroll; ++k)
-        if (v0 + k * kLpThreads >= piece.end) q[k] = make_uint4(none, none, none, none);
+        if (v0 + k * NT >= piece.end) q[k] = make_uint4(low, low, low, low);
     }
-    sm.raise(mx);
-    const float minus = -sm.ref();
+    const float minus = -origin(sm.m);
     const uint64_t off = f32x2(minus, minus), scale = f32x2(kLog2e, kLog2e);
     uint64_t z = 0, s = 0;  // (0.f, 0.f)
 #pragma unroll
@@ -380,39 +418,39 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(
 #pragma unroll
       for (int i = 0; i < Row<T>::kVec / 2; ++i) {
         const float2 x = pair(q[k], i, row.x);
-        const float2 y = unpack(mul2(add2(f32x2(x.x, x.y), off), scale));
-        const float y0 = floor_exponent(y.x), y1 = floor_exponent(y.y);
-        const uint64_t e = f32x2(ex2(y0), ex2(y1));
+        const uint64_t y = fma2(f32x2(x.x, x.y), scale, off);  // at least -3 kHuge: 2^y y is finite
+        const float2 yy = unpack(y);
+        const uint64_t e = f32x2(ex2(yy.x), ex2(yy.y));
         z = add2(z, e);
-        s = fma2(e, f32x2(y0, y1), s);
+        s = fma2(e, y, s);
       }
     }
     const float2 zz = unpack(z), ss = unpack(s);
     sm.z += zz.x + zz.y;
     sm.s += ss.x + ss.y;
+  };
+  uint4 even[kUnroll], odd[kUnroll];
+  load(even, piece.begin + tid);
+  for (int v0 = piece.begin + tid; v0 < piece.end; v0 += 2 * kUnroll * NT) {
+    load(odd, v0 + kUnroll * NT);
+    sum_batch(even, v0);
+    load(even, v0 + 2 * kUnroll * NT);
+    sum_batch(odd, v0 + kUnroll * NT);
   }
   // ---- the block's sums
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    Softmax other;
-    other.m = __shfl_xor_sync(0xffffffffu, sm.m, o);
-    other.z = __shfl_xor_sync(0xffffffffu, sm.z, o);
-    other.s = __shfl_xor_sync(0xffffffffu, sm.s, o);
-    sm.merge(other);
-  }
+  sm = warp_merge(sm, 32);
   if (lane == 0) sh.parts[warp] = sm;
   if (top_n > 0) block_top(piece, top_n, any ? logit_key(thread_max) : 0u, sh);
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kLpWarps; ++w) sm.merge(sh.parts[w]);
-    sh.sum = sm;
+  if (warp == 0) {
+    sm = warp_merge(sh.parts[lane % (NT / 32)], (NT / 32));
+    if (lane == 0) sh.sum = sm;
   }
   if (blocks > 1) {
     cluster.sync();
+    const int n = blocks * top_n;
     if (rank == 0) {
-      if (tid == 0)
-        for (int b = 1; b < blocks; ++b) sm.merge(*cluster.map_shared_rank(&sh.sum, b));
-      const int n = blocks * top_n;
+      if (warp == 0) sm = warp_merge(*cluster.map_shared_rank(&sh.sum, lane % blocks), blocks);
       if (tid < n) sh.all[tid] = cluster.map_shared_rank(sh.top, tid / top_n)[tid % top_n];
     }
     cluster.sync();  // the others' shared memory has been read
@@ -420,7 +458,6 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(
     if (tid == 0) sh.sum = sm;
     if (tid < kMaxTop) sh.top[tid] = 0;
     __syncthreads();
-    const int n = blocks * top_n;
     if (tid < n && sh.all[tid] != 0) {
       const uint64_t e = sh.all[tid];
       int r = 0;
@@ -435,11 +472,11 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(
   const bool masked = sum.m == -INFINITY && sum.z == sum.z;  // every logit is -inf
   auto logprob = [&](float x) {
     if (x == -INFINITY && sum.z == sum.z) return -INFINITY;
-    return ((x - sum.m) * kLog2e - log_z) * kLn2;
+    if (x > -kHuge && fabsf(sum.m) < kHuge) return (fmaf(x, kLog2e, -origin(sum.m)) - log_z) * kLn2;
+    return (x - sum.m) - log_z * kLn2;  // for a usual m: log z and its origin are below the rounding of x
   };
   if (tid == 0) {
-    const int64_t t = tokens[row_at];
-    logprobs[row_at] = logprob(t >= 0 && t < vocab ? load_logit(row.x + t) : -INFINITY);
+    logprobs[row_at] = logprob(asked);
     entropies[row_at] = masked ? 0.f : (log_z - sum.s / sum.z) * kLn2;
   }
   if (tid < top_n) {
@@ -449,17 +486,13 @@ __global__ void __launch_bounds__(kLpThreads, 3) token_logprobs_kernel(
   }
 }
 
-template <typename T>
-cudaError_t launch_logprobs(const void* logits, int64_t row_stride, int64_t rows, int vocab, const int64_t* tokens, int top_n,
-                            float* logprobs, float* entropies, int64_t* top_tokens, float* top_logprobs, cudaStream_t stream) {
-  // Blocks per row: enough that three blocks an SM are busy, as long as a thread keeps a full batch of loads.
-  int blocks = 1;
-  while (blocks < kMaxCluster && rows * blocks < 3 * 148 &&
-         vocab / (2 * blocks) >= kLpThreads * kUnroll * Row<T>::kVec / 2)
-    blocks *= 2;
+template <typename T, int NT>
+cudaError_t launch_logprobs_blocks(int blocks, const void* logits, int64_t row_stride, int64_t rows, int vocab,
+                                   const int64_t* tokens, int top_n, float* logprobs, float* entropies,
+                                   int64_t* top_tokens, float* top_logprobs, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(rows * blocks));
-  cfg.blockDim = dim3(kLpThreads);
+  cfg.blockDim = dim3(NT);
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -467,8 +500,16 @@ cudaError_t launch_logprobs(const void* logits, int64_t row_stride, int64_t rows
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, static_cast<const T*>(logits), row_stride, vocab, tokens,
-                            top_n, logprobs, entropies, top_tokens, top_logprobs);
+  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT>, static_cast<const T*>(logits), row_stride, vocab,
+                            tokens, top_n, logprobs, entropies, top_tokens, top_logprobs);
+}
+
+template <typename T, typename... Args>
+cudaError_t launch_logprobs(const void* logits, int64_t row_stride, int64_t rows, int vocab, Args... args) {
+  int blocks = 1;
+  while (blocks < kMaxCluster && rows * blocks < 148 && vocab / (2 * blocks) >= 512 * kUnroll * Row<T>::kVec / 2) blocks *= 2;
+  if (rows >= 4 * 148) return launch_logprobs_blocks<T, 256>(blocks, logits, row_stride, rows, vocab, args...);
+  return launch_logprobs_blocks<T, 512>(blocks, logits, row_stride, rows, vocab, args...);
 }
 
 }  // namespace
