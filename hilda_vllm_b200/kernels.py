@@ -434,11 +434,13 @@ def argmax_shard(logits: torch.Tensor, index_offset: int, out_tokens: torch.Tens
 # ------------------------------------------------------------------------ page tables
 def _on_one_device(first: torch.Tensor, *rest: torch.Tensor) -> None:
     """All tensors (None allowed) on one CUDA device."""
-    _cuda(first, *rest)
     dev = first.get_device()
     for t in rest:
         if t is not None and t.get_device() != dev:
+            _cuda(first, *rest)
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    if dev < 0:
+        _cuda(first)
 
 
 def _launch(name: str, t: torch.Tensor, *args) -> None:

@@ -259,7 +259,7 @@ def test_store_blocks_skips_what_has_no_place():
     kc, ks = pool(g, 4, 256, 2, 64)
     vc, vs = pool(g, 4, 256, 2, 64)
     state = [t.to(DEV) for t in (kc, vc, ks, vs)]
-    tables = [[0, 1], [-1, -1], [4, 3], [3, 2 ** 31 - 1], [2, 2]]
+    tables = [[0, 1], [-1, -1], [4, 3], [1, 2 ** 31 - 1], [2, 2]]  # no page is written by two sequences
     context, query = [0, 5, 300, 600, 3], [1, 5, 300, 600, 7]
     cu = np.concatenate(([0], np.cumsum(query))).tolist()
     x = torch.randn(cu[-1], 2, D, generator=g).bfloat16()
