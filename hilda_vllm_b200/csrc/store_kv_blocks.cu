@@ -11,19 +11,19 @@
 // held for an earlier owner.
 //
 // The rows of a call that fall into one group are a run, and consecutive rows.  A thread block looks
-// for the runs that start in its window of rows, for one head and K or V.  A run of up to 16 rows is
-// one warp's, a longer one the whole block's; either way the rows are loaded once, all loads in
-// flight together, and stay in registers between the maximum and the rounding.  HBM bounds long runs
-// (3 B an element), the chain of reads (sequence, table, scale) a decode step.
+// for the runs that start in its window of rows and stores them for several items, an item being one
+// head of K or of V.  A warp holds up to 2 L rows of an item in registers between the maximum and the rounding, L loads a lane in flight, and no warp waits
+// for another but for the maximum of a longer run, which two or four warps share.  HBM bounds a
+// prefill (3 B an element): L = 32, twelve warps of 16 KB an SM.  A decode step is bound by its chain
+// of reads (sequence, table, scale): L = 8, more and smaller warps.
 #include "kv_blocks.cuh"
 
 namespace hl {
 namespace {
 
-constexpr int kStoreThreads = 256;
+constexpr int kStoreThreads = 128;
 constexpr int kStoreWarps = kStoreThreads / 32;
-constexpr int kMaxWindow = 64;
-constexpr int kWarpRun = 16;         // longest run of one warp
+constexpr int kMaxWindow = 256;
 constexpr int kMaxSharedSeqs = 4096; // cu_seqlens_q of up to so many sequences is searched in shared memory
 
 struct StoreBlocksParams {
@@ -43,19 +43,20 @@ struct StoreBlocksParams {
   int scale_block;
   int64_t num_blocks;
   int window;  // rows whose runs one thread block starts
+  int items;   // heads of K and V that it stores, of 2 Hk
 };
 
 // The rows of a call that fall into one group: rows [row, row + count) go to offsets
 // [held, held + count) of the group whose first slot is `slot0`.  count = 0: none.
 struct GroupRun {
-  int64_t row, slot0;
+  int64_t row, slot0, group;  // group: slot0 / scale_block
   int count, held;
 };
 
 // The run that starts at row i; count 0 where i is inside a run or belongs to no sequence.
 // cu: the prefix sums, or nullptr for one row per sequence.
 __device__ GroupRun run_at(const StoreBlocksParams& p, const int32_t* cu, int64_t i) {
-  GroupRun r{i, 0, 0, 0};
+  GroupRun r{i, 0, 0, 0, 0};
   int64_t first = i, end = i + 1;  // rows of i's sequence
   int b = int(i);
   if (cu) {
@@ -80,31 +81,43 @@ __device__ GroupRun run_at(const StoreBlocksParams& p, const int32_t* cu, int64_
   if (page < 0 || page >= p.num_blocks) return r;
   r.held = int(held);
   r.slot0 = page * p.block_size + off - held;
+  r.group = page * (p.block_size / p.scale_block) + off / unsigned(p.scale_block);
   r.count = int(min(int64_t(p.scale_block) - held, min(end, p.num_tokens) - i));
   return r;
 }
 
-// Largest finite |x| of a vector, as a bf16 bit pattern; patterns from 0x7f80 on are infinities and NaN.
-__device__ __forceinline__ uint32_t abs_bits(uint4 v) {
-  return __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+// Running maximum of |x| over pairs of bf16 values: NaN is passed over, infinities are not.
+__device__ __forceinline__ void raise_abs(__nv_bfloat162& m, uint4 v) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) m = __hmax2(m, __habs2(h[t]));
 }
-__device__ __forceinline__ uint32_t finite_bits(uint4 v) {
+// The same over finite values only.
+__device__ __forceinline__ void raise_finite(__nv_bfloat162& m, uint4 v) {
   auto keep = [](uint32_t w) {
-    w &= 0x7fff7fffu;
-    if ((w & 0xffffu) >= 0x7f80u) w &= 0xffff0000u;
-    if ((w >> 16) >= 0x7f80u) w &= 0xffffu;
+    if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+    if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
     return w;
   };
-  return __vmaxu2(__vmaxu2(keep(v.x), keep(v.y)), __vmaxu2(keep(v.z), keep(v.w)));
+  raise_abs(m, make_uint4(keep(v.x), keep(v.y), keep(v.z), keep(v.w)));
 }
-__device__ __forceinline__ uint32_t larger_half(uint32_t w) { return max(w & 0xffffu, w >> 16); }
+// Larger half of the warp's maxima, as bits: at least 0x7f80 if a value is infinite.
+__device__ __forceinline__ uint32_t warp_max_bits(__nv_bfloat162 m) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(&m);
+  return __reduce_max_sync(0xffffffffu, max(w & 0xffffu, w >> 16));
+}
 
-__device__ __forceinline__ uint2 scale_to_e4m3(uint4 v, float inverse) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// e4m3(x * inverse), inverse a power of two: exact in bf16 but for results below 2^-126, which round to
+// zero either way.
+__device__ __forceinline__ uint2 scale_to_e4m3(uint4 v, __nv_bfloat162 inverse) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
   uint32_t q[4];
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
-    q[t] = __nv_cvt_float2_to_fp8x2(make_float2(bf16lo(w[t]) * inverse, bf16hi(w[t]) * inverse), __NV_SATFINITE, __NV_E4M3);
+  for (int t = 0; t < 4; ++t) {
+    const __nv_bfloat162 y = __hmul2(h[t], inverse);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&y);
+    q[t] = __nv_cvt_float2_to_fp8x2(make_float2(bf16lo(w), bf16hi(w)), __NV_SATFINITE, __NV_E4M3);
+  }
   return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
 }
 
@@ -130,7 +143,7 @@ struct RunPlace {
   __device__ RunPlace(const StoreBlocksParams& p, const GroupRun& r, int kv, int head)
       : x(p.x[kv] + r.row * p.x_stride[kv] + head * kBlockHeadDim),
         out(p.cache[kv] + (r.slot0 * p.num_kv_heads + head) * kBlockHeadDim),
-        scale(p.scales[kv] + r.slot0 / p.scale_block * p.num_kv_heads + head) {}
+        scale(p.scales[kv] + r.group * p.num_kv_heads + head) {}
 };
 
 // The group's new scale from the largest new value and the old scale (ignored unless rows are held);
@@ -145,116 +158,113 @@ __device__ __forceinline__ float new_scale(uint32_t amax_bits, bool held, float 
   return s;
 }
 // 1 / s of a power of two between 2^-100 and 2^126.
-__device__ __forceinline__ float inverse_pow2(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
-
-// One warp, a run of at most kWarpRun rows: 16 lanes per row.
-__device__ void store_warp_run(const StoreBlocksParams& p, const GroupRun& r, int kv, int head, int lane) {
-  const RunPlace at(p, r, kv, head);
-  const int row = lane >> 4, e0 = (lane & 15) * 8;
-  const int64_t row_bytes = int64_t(p.num_kv_heads) * kBlockHeadDim;
-  const float old = r.held ? *at.scale : 0.f;
-  uint4 v[kWarpRun / 2];
-#pragma unroll
-  for (int k = 0; k < kWarpRun / 2; ++k)
-    v[k] = 2 * k + row < r.count ? __ldg(reinterpret_cast<const uint4*>(at.x + (2 * k + row) * p.x_stride[kv] + e0))
-                                 : make_uint4(0, 0, 0, 0);
-  uint32_t m = 0;
-#pragma unroll
-  for (int k = 0; k < kWarpRun / 2; ++k) m = __vmaxu2(m, abs_bits(v[k]));
-  uint32_t amax = __reduce_max_sync(0xffffffffu, larger_half(m));
-  if (amax >= 0x7f80u) {
-    m = 0;
-#pragma unroll
-    for (int k = 0; k < kWarpRun / 2; ++k) m = __vmaxu2(m, finite_bits(v[k]));
-    amax = __reduce_max_sync(0xffffffffu, larger_half(m));
-  }
-  float ratio;
-  const float s = new_scale(amax, r.held > 0, old, ratio), inverse = inverse_pow2(s);
-#pragma unroll
-  for (int k = 0; k < kWarpRun / 2; ++k)
-    if (2 * k + row < r.count)
-      *reinterpret_cast<uint2*>(at.out + (r.held + 2 * k + row) * row_bytes + e0) = scale_to_e4m3(v[k], inverse);
-  if (ratio != 1.f) rescale_rows(at.out + e0, row_bytes, r.held, ratio, row, 2);
-  if (lane == 0) *at.scale = s;
+__device__ __forceinline__ __nv_bfloat162 inverse_pow2(float s) {
+  return __float2bfloat162_rn(__uint_as_float((254u << 23) - __float_as_uint(s)));
 }
 
-// The whole block, a longer run: 16 rows a pass, up to P passes in registers; what is longer is read
-// twice.
-template <int P>
-__device__ void store_block_run(const StoreBlocksParams& p, const GroupRun& r, int kv, int head, uint32_t* warp_max) {
+// M warps, one run of one item: warp `sub` of them holds rows 2 L sub .. 2 L (sub + 1) - 1, two a load; of
+// a run that is longer than 2 L M rows the same of every 2 L M, which are then read twice.
+template <int M, int L>
+__device__ __forceinline__ void store_run(const StoreBlocksParams& p, const GroupRun& r, int kv, int head, int sub,
+                                               int team, int lane, uint32_t* team_max) {
+  constexpr int kHeldRows = 2 * L;
   const RunPlace at(p, r, kv, head);
-  const int row = threadIdx.x >> 4, e0 = (threadIdx.x & 15) * 8;
-  const int64_t row_bytes = int64_t(p.num_kv_heads) * kBlockHeadDim;
+  const int row = sub * kHeldRows + (lane >> 4), e0 = (lane & 15) * 8;
+  const int64_t row_bytes = int64_t(p.num_kv_heads) * kBlockHeadDim, step = 2 * p.x_stride[kv];
   const float old = r.held ? *at.scale : 0.f;
-  constexpr int kRows = kStoreThreads / 16;
-  uint4 v[P];
+  const bool twice = r.count > M * kHeldRows;
+  uint4 v[L];
   auto load = [&](int i0) {
+    const __nv_bfloat16* x = at.x + (i0 + row) * p.x_stride[kv] + e0;
+    if (i0 + (sub + 1) * kHeldRows <= r.count) {
 #pragma unroll
-    for (int k = 0; k < P; ++k)
-      v[k] = i0 + k * kRows + row < r.count
-                 ? __ldg(reinterpret_cast<const uint4*>(at.x + (i0 + k * kRows + row) * p.x_stride[kv] + e0))
-                 : make_uint4(0, 0, 0, 0);
-  };
-  auto block_max = [&](uint32_t m) {
-    m = __reduce_max_sync(0xffffffffu, larger_half(m));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = 0;
+      for (int k = 0; k < L; ++k) v[k] = __ldg(reinterpret_cast<const uint4*>(x + k * step));
+    } else {
 #pragma unroll
-    for (int w = 0; w < kStoreWarps; ++w) m = max(m, warp_max[w]);
-    return m;
-  };
-  auto run_max = [&](auto bits) {
-    uint32_t m = 0;
-    for (int i0 = 0; i0 < r.count; i0 += P * kRows) {
-      if (i0 > 0 || r.count > P * kRows) load(i0);
-#pragma unroll
-      for (int k = 0; k < P; ++k) m = __vmaxu2(m, bits(v[k]));
+      for (int k = 0; k < L; ++k)
+        v[k] = i0 + row + 2 * k < r.count ? __ldg(reinterpret_cast<const uint4*>(x + k * step)) : make_uint4(0, 0, 0, 0);
     }
-    return block_max(m);
   };
-  load(0);
-  uint32_t amax = run_max([](uint4 x) { return abs_bits(x); });
-  if (amax >= 0x7f80u) amax = run_max([](uint4 x) { return finite_bits(x); });
-  float ratio;
-  const float s = new_scale(amax, r.held > 0, old, ratio), inverse = inverse_pow2(s);
-  for (int i0 = 0; i0 < r.count; i0 += P * kRows) {
-    if (r.count > P * kRows) load(i0);
+  auto run_max = [&](auto raise) {
+    __nv_bfloat162 m = __float2bfloat162_rn(0.f);
+    for (int i0 = 0; i0 < r.count; i0 += M * kHeldRows) {
+      if (twice) load(i0);
 #pragma unroll
-    for (int k = 0; k < P; ++k)
-      if (i0 + k * kRows + row < r.count)
-        *reinterpret_cast<uint2*>(at.out + (r.held + i0 + k * kRows + row) * row_bytes + e0) = scale_to_e4m3(v[k], inverse);
+      for (int k = 0; k < L; ++k) raise(m, v[k]);
+    }
+    uint32_t w = warp_max_bits(m);
+    if constexpr (M > 1) {
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * M) : "memory");  // the last maxima have been read
+      if (lane == 0) team_max[sub] = w;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * M) : "memory");
+#pragma unroll
+      for (int i = 0; i < M; ++i) w = max(w, team_max[i]);
+    }
+    return w;
+  };
+  if (!twice) load(0);
+  uint32_t amax = run_max([](__nv_bfloat162& m, uint4 x) { raise_abs(m, x); });
+  if (amax >= 0x7f80u) amax = run_max([](__nv_bfloat162& m, uint4 x) { raise_finite(m, x); });
+  float ratio;
+  const float s = new_scale(amax, r.held > 0, old, ratio);
+  const __nv_bfloat162 inverse = inverse_pow2(s);
+  for (int i0 = 0; i0 < r.count; i0 += M * kHeldRows) {
+    if (twice) load(i0);
+    uint8_t* out = at.out + (r.held + i0 + row) * row_bytes + e0;
+#pragma unroll
+    for (int k = 0; k < L; ++k)
+      if (i0 + row + 2 * k < r.count) *reinterpret_cast<uint2*>(out + 2 * k * row_bytes) = scale_to_e4m3(v[k], inverse);
   }
-  if (ratio != 1.f) rescale_rows(at.out + e0, row_bytes, r.held, ratio, row, kRows);
-  if (threadIdx.x == 0) *at.scale = s;
+  if (ratio != 1.f) rescale_rows(at.out + e0, row_bytes, r.held, ratio, 2 * sub + (lane >> 4), 2 * M);
+  if (sub == 0 && lane == 0) *at.scale = s;
 }
 
-template <int P>
-__global__ void __launch_bounds__(kStoreThreads) store_kv_blocks_kernel(const __grid_constant__ StoreBlocksParams p) {
+template <int M, int L>
+__global__ void __launch_bounds__(kStoreThreads, L > 8 ? 3 : 8) store_kv_blocks_kernel(const __grid_constant__ StoreBlocksParams p) {
   extern __shared__ int32_t cu_shared[];
   __shared__ GroupRun runs[kMaxWindow];
-  __shared__ int small[kMaxWindow], large[kMaxWindow], num_small, num_large;
-  __shared__ uint32_t warp_max[kStoreWarps];
-  const int kv = blockIdx.z, head = blockIdx.y;
+  __shared__ int found[kMaxWindow], num_found;
+  __shared__ uint32_t team_max[kStoreWarps / M][M];
+  const int item0 = blockIdx.y * p.items, items = min(p.items, 2 * p.num_kv_heads - item0);
   const int64_t begin = int64_t(blockIdx.x) * p.window;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int32_t* cu = p.cu;
   if (cu && p.num_seqs <= kMaxSharedSeqs) {
     for (int i = threadIdx.x; i <= p.num_seqs; i += kStoreThreads) cu_shared[i] = cu[i];
     cu = cu_shared;
   }
-  if (threadIdx.x == 0) num_small = num_large = 0;
+  const int window = int(min(int64_t(p.window), p.num_tokens - begin));
+  if (threadIdx.x == 0) num_found = 0;
   __syncthreads();
-  if (threadIdx.x < p.window && begin + threadIdx.x < p.num_tokens) {
-    const GroupRun r = run_at(p, cu, begin + threadIdx.x);
-    runs[threadIdx.x] = r;
-    if (r.count > kWarpRun) large[atomicAdd(&num_large, 1)] = threadIdx.x;
-    else if (r.count > 0) small[atomicAdd(&num_small, 1)] = threadIdx.x;
+  for (int i = threadIdx.x; i < window; i += kStoreThreads) {
+    const GroupRun r = run_at(p, cu, begin + i);
+    runs[i] = r;
+    if (r.count > 0) found[atomicAdd(&num_found, 1)] = i;
   }
   __syncthreads();
-  for (int i = threadIdx.x >> 5; i < num_small; i += kStoreWarps)
-    store_warp_run(p, runs[small[i]], kv, head, threadIdx.x & 31);
-  for (int i = 0; i < num_large; ++i) store_block_run<P>(p, runs[large[i]], kv, head, warp_max);
+  for (int i = warp / M; i < num_found * items; i += kStoreWarps / M) {
+    const int item = item0 + i % items;
+    store_run<M, L>(p, runs[found[i / items]], item & 1, item >> 1, warp % M, warp / M, lane, team_max[warp / M]);
+  }
+}
+
+template <int M, int L>
+void launch_store_blocks(StoreBlocksParams& p, int64_t window, int64_t items, cudaStream_t stream) {
+  p.window = int(window);
+  p.items = int(items);
+  const dim3 grid(unsigned((p.num_tokens + window - 1) / window), unsigned((2 * p.num_kv_heads + items - 1) / items));
+  const size_t shared = p.cu && p.num_seqs <= kMaxSharedSeqs ? (p.num_seqs + 1) * sizeof(int32_t) : 0;
+  store_kv_blocks_kernel<M, L><<<grid, kStoreThreads, shared, stream>>>(p);
+}
+
+// Windows of a group's rows, which start about one run each, and an item at least for each team of M
+// warps, more where that still makes twelve blocks an SM.
+template <int M>
+void launch_store_prefill(StoreBlocksParams& p, cudaStream_t stream) {
+  const int64_t window = p.scale_block < kMaxWindow ? p.scale_block : kMaxWindow, all = 2 * int64_t(p.num_kv_heads);
+  const int64_t teams = kStoreWarps / M, blocks = (p.num_tokens + window - 1) / window * all / (12 * 148);
+  const int64_t items = blocks > teams ? blocks / teams * teams : teams;
+  launch_store_blocks<M, 32>(p, window, items < all ? items : all, stream);
 }
 
 }  // namespace
@@ -272,7 +282,7 @@ extern "C" int hl_store_kv_fp8_blocks(const void* key, const void* value, int64_
   HL_CHECK_ARG(num_tokens >= 0 && num_tokens <= 0x7fffffff && num_seqs >= 0,
                "hl_store_kv_fp8_blocks: num_tokens or num_seqs out of range");
   HL_CHECK_ARG(head_dim == kBlockHeadDim, "hl_store_kv_fp8_blocks: head_dim %d != 128", head_dim);
-  HL_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 65535, "hl_store_kv_fp8_blocks: bad num_kv_heads");
+  HL_CHECK_ARG(num_kv_heads > 0 && num_kv_heads <= 32767, "hl_store_kv_fp8_blocks: bad num_kv_heads");
   HL_CHECK_ARG(scale_block > 0 && scale_block % 64 == 0 && block_size > 0 && block_size % scale_block == 0,
                "hl_store_kv_fp8_blocks: scale_block must be a multiple of 64 that divides block_size");
   HL_CHECK_ARG(cu_seqlens_q || num_tokens == num_seqs,
@@ -307,19 +317,17 @@ extern "C" int hl_store_kv_fp8_blocks(const void* key, const void* value, int64_
   p.block_size = block_size;
   p.scale_block = scale_block;
   p.num_blocks = num_blocks;
-  // Windows of 64 rows, which start about one run each in a prefill; of 8, a warp for each row of a
-  // decode step, where those would leave SMs idle.
-  const int64_t wide = (num_tokens + kMaxWindow - 1) / kMaxWindow;
-  p.window = wide * num_kv_heads * 2 >= 2 * 148 ? kMaxWindow : kStoreWarps;
-  const dim3 grid(unsigned((num_tokens + p.window - 1) / p.window), num_kv_heads, 2);
-  const size_t shared = cu_seqlens_q && num_seqs <= kMaxSharedSeqs ? (num_seqs + 1) * sizeof(int32_t) : 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (scale_block <= 64)
-    store_kv_blocks_kernel<4><<<grid, kStoreThreads, shared, s>>>(p);
+  // Fewer than four rows a sequence: a warp for each row and item (256 x 1 row, 8 heads: 6.6 us, with
+  // the prefill kernel 12.3 us).
+  if (num_tokens < 4 * int64_t(num_seqs))
+    launch_store_blocks<1, 8>(p, kStoreWarps, 1, s);
+  else if (scale_block <= 64)
+    launch_store_prefill<1>(p, s);
   else if (scale_block <= 128)
-    store_kv_blocks_kernel<8><<<grid, kStoreThreads, shared, s>>>(p);
+    launch_store_prefill<2>(p, s);
   else
-    store_kv_blocks_kernel<16><<<grid, kStoreThreads, shared, s>>>(p);
+    launch_store_prefill<4>(p, s);
   HL_CHECK_LAUNCH("hl_store_kv_fp8_blocks");
   return HL_OK;
 }
