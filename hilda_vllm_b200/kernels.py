@@ -432,6 +432,11 @@ def argmax_shard(logits: torch.Tensor, index_offset: int, out_tokens: torch.Tens
 
 
 # ------------------------------------------------------------------------ page tables
+# The checks of the operators below are written to be cheap (one stride() or shape per tensor): their
+# small calls take less time on the GPU than on the host.
+_BF16, _F32, _E4M3, _I32, _I64 = torch.bfloat16, torch.float32, torch.float8_e4m3fn, torch.int32, torch.int64
+
+
 def _on_one_device(first: torch.Tensor, *rest: torch.Tensor) -> None:
     """All tensors (None allowed) on one CUDA device."""
     dev = first.get_device()
@@ -447,7 +452,7 @@ def _launch(name: str, t: torch.Tensor, *args) -> None:
     """Calls the C entry point `name` on t's device, current or not, and that device's stream."""
     fn = getattr(_lib.load(), name)
     dev = t.get_device()
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)), name)
     else:
         with torch.cuda.device(dev):
@@ -467,23 +472,24 @@ def extend_block_tables(block_tables: torch.Tensor, cached_lens: torch.Tensor | 
     max_tokens entries, 0 / -1 behind the batch's last token) plus context_lens and status, int32
     [2]: pages taken, error bits (1: free list too short, 2: table too narrow, 4: more than
     max_tokens tokens; what did not fit is -1)."""
-    _on_one_device(block_tables, cached_lens, query_lens, free_blocks)
+    _on_one_device(block_tables, query_lens, free_blocks, cached_lens)
     b, width = block_tables.shape
-    assert block_tables.dtype == torch.int32 and block_tables.stride(1) == 1
-    assert query_lens.dtype == torch.int32 and query_lens.is_contiguous() and query_lens.shape == (b,)
-    if cached_lens is not None:
-        assert cached_lens.dtype == torch.int32 and cached_lens.is_contiguous() and cached_lens.shape == (b,)
-    assert free_blocks.dtype == torch.int32 and free_blocks.is_contiguous() and free_blocks.dim() == 1
+    row, one = block_tables.stride()
+    assert block_tables.dtype == _I32 and one == 1
+    assert query_lens.dtype == _I32 and query_lens.is_contiguous() and query_lens.shape == (b,)
+    assert cached_lens is None or (cached_lens.dtype == _I32 and cached_lens.is_contiguous()
+                                   and cached_lens.shape == (b,))
+    assert free_blocks.dtype == _I32 and free_blocks.is_contiguous() and free_blocks.dim() == 1
     dev = block_tables.device
     # One allocation for the int32 results (slots first: 16-byte stores), one for the positions.
-    slots, cu_q, cu_k, context, status = torch.empty(max_tokens + 3 * b + 4, dtype=torch.int32, device=dev).split(
-        (max_tokens, b + 1, b + 1, b, 2))
-    positions = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+    slots, cu_q, cu_k, context, status = torch.empty(
+        max_tokens + 3 * b + 4, dtype=_I32, device=dev).split_with_sizes((max_tokens, b + 1, b + 1, b, 2))
+    positions = torch.empty(max_tokens, dtype=_I64, device=dev)
     _launch(
-        "hl_extend_block_tables", block_tables, _p(cached_lens), query_lens.data_ptr(), b, block_tables.data_ptr(),
-        block_tables.stride(0), width, free_blocks.data_ptr(), free_blocks.numel(), int(block_size), int(max_tokens),
-        cu_q.data_ptr(), cu_k.data_ptr(), context.data_ptr(), positions.data_ptr(), slots.data_ptr(),
-        status.data_ptr())
+        "hl_extend_block_tables", block_tables, None if cached_lens is None else cached_lens.data_ptr(),
+        query_lens.data_ptr(), b, block_tables.data_ptr(), row, width, free_blocks.data_ptr(), free_blocks.numel(),
+        block_size, max_tokens, cu_q.data_ptr(), cu_k.data_ptr(), context.data_ptr(), positions.data_ptr(),
+        slots.data_ptr(), status.data_ptr())
     return {"block_tables": block_tables, "cu_seqlens_q": cu_q, "cu_seqlens_k": cu_k, "context_lens": context,
             "positions": positions, "slot_mapping": slots, "status": status}
 
@@ -491,13 +497,14 @@ def extend_block_tables(block_tables: torch.Tensor, cached_lens: torch.Tensor | 
 # ------------------------------------------------------------------------ block-scaled 8-bit cache
 def _check_block_cache(k_cache, v_cache, k_scales, v_scales):
     """(num_blocks, block_size, Hk, D, scale_block) of a block-scaled cache."""
-    nb, bs, hk, d = k_cache.shape
-    assert k_cache.dtype == torch.float8_e4m3fn and v_cache.dtype == torch.float8_e4m3fn
-    assert k_cache.is_contiguous() and v_cache.is_contiguous() and v_cache.shape == k_cache.shape
-    assert k_scales.dtype == torch.float32 and v_scales.dtype == torch.float32
-    assert k_scales.is_contiguous() and v_scales.is_contiguous() and v_scales.shape == k_scales.shape
-    groups = k_scales.shape[1]
-    assert k_scales.shape == (nb, groups, hk) and groups > 0 and bs % groups == 0
+    shape, scales = k_cache.shape, k_scales.shape
+    nb, bs, hk, d = shape
+    snb, groups, shk = scales
+    assert k_cache.dtype == _E4M3 == v_cache.dtype and v_cache.shape == shape
+    assert k_scales.dtype == _F32 == v_scales.dtype and v_scales.shape == scales
+    assert (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous()
+            and v_scales.is_contiguous())
+    assert snb == nb and shk == hk and groups > 0 and bs % groups == 0
     return nb, bs, hk, d, bs // groups
 
 
@@ -513,23 +520,29 @@ def store_kvcache_fp8_blocks(key: torch.Tensor, value: torch.Tensor, k_cache: to
     per sequence).  Tokens that a block held before are rescaled when its scale grows; whatever a
     page held for an earlier owner does not count."""
     _on_one_device(key, value, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, cu_seqlens_q)
-    n, hk, hd = key.shape
+    shape = key.shape
+    n, hk, hd = shape
     nb, bs, hk2, hd2, t = _check_block_cache(k_cache, v_cache, k_scales, v_scales)
-    assert value.shape == key.shape and (hk, hd) == (hk2, hd2)
-    assert key.dtype == torch.bfloat16 and value.dtype == torch.bfloat16
-    assert n == 0 or (key.stride(2) == 1 and value.stride(2) == 1 and key.stride(1) == hd and value.stride(1) == hd)
-    assert block_tables.dtype == torch.int32 and block_tables.stride(1) == 1
-    assert context_lens.dtype == torch.int32 and context_lens.is_contiguous()
+    assert value.shape == shape and hk == hk2 and hd == hd2
+    assert key.dtype == _BF16 == value.dtype
+    krs, khs, kes = key.stride()
+    vrs, vhs, ves = value.stride()
+    assert n == 0 or (kes == 1 == ves and khs == hd == vhs)
+    rows, width = block_tables.shape
+    row, one = block_tables.stride()
     b = context_lens.numel()
-    assert block_tables.shape[0] >= b
+    assert block_tables.dtype == _I32 and one == 1 and rows >= b
+    assert context_lens.dtype == _I32 and context_lens.is_contiguous()
+    cu = None
     if cu_seqlens_q is not None:
-        assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.numel() == b + 1
-    # One row may come with any row stride (a slice of a single-row tensor).
-    krs, vrs = (key.stride(0), value.stride(0)) if n > 1 else (hk * hd, hk * hd)
+        assert cu_seqlens_q.dtype == _I32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.numel() == b + 1
+        cu = cu_seqlens_q.data_ptr()
+    if n <= 1:  # a single row may come with any row stride
+        krs = vrs = hk * hd
     _launch(
         "hl_store_kv_fp8_blocks", key, key.data_ptr(), value.data_ptr(), krs, vrs, n, k_cache.data_ptr(),
-        v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-        block_tables.shape[1], context_lens.data_ptr(), _p(cu_seqlens_q), b, hk, hd, bs, t, nb)
+        v_cache.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(), row, width,
+        context_lens.data_ptr(), cu, b, hk, hd, bs, t, nb)
 
 
 def make_block_decode_workspace(batch: int, num_q_heads: int, num_kv_heads: int, device) -> torch.Tensor:
@@ -551,26 +564,32 @@ def paged_decode_fp8_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         assert q.shape[1] == 1
         q = q.squeeze(1)
     _on_one_device(q, k_cache, v_cache, k_scales, v_scales, block_tables, context_lens, out, workspace)
-    b, hq, hd = q.shape
+    shape = q.shape
+    b, hq, hd = shape
     nb, bs, hk, hd2, t = _check_block_cache(k_cache, v_cache, k_scales, v_scales)
-    assert q.dtype == torch.bfloat16 and hd == hd2
-    assert b == 0 or (q.stride(2) == 1 and q.stride(1) == hd)
-    assert block_tables.dtype == torch.int32 and block_tables.stride(1) == 1 and block_tables.shape[0] >= b
-    assert context_lens.dtype == torch.int32 and context_lens.is_contiguous() and context_lens.numel() >= b
+    qrs, qhs, qes = q.stride()
+    assert q.dtype == _BF16 and hd == hd2 and (b == 0 or (qes == 1 and qhs == hd))
+    rows, width = block_tables.shape
+    row, one = block_tables.stride()
+    assert block_tables.dtype == _I32 and one == 1 and rows >= b
+    assert context_lens.dtype == _I32 and context_lens.is_contiguous() and context_lens.numel() >= b
+    ors = hq * hd
     if out is None:
-        out = torch.empty(b, hq, hd, dtype=torch.bfloat16, device=q.device)
-    assert out.dtype == torch.bfloat16 and out.shape == (b, hq, hd) and out.stride(2) == 1 and out.stride(1) == hd
+        out = torch.empty(shape, dtype=_BF16, device=q.device)
+    else:
+        ors, ohs, oes = out.stride()
+        assert out.dtype == _BF16 and out.shape == shape and (b == 0 or (oes == 1 and ohs == hd))
     if b == 0:
         return out
     if workspace is None:
         workspace = make_block_decode_workspace(b, hq, hk, q.device)
     assert workspace.dtype == torch.uint8 and workspace.is_contiguous()
-    qrs, ors = (q.stride(0), out.stride(0)) if b > 1 else (hq * hd, hq * hd)
+    if b == 1:  # a single row may come with any row stride
+        qrs = ors = hq * hd
     _launch(
         "hl_paged_decode_fp8_blocks", q, q.data_ptr(), qrs, k_cache.data_ptr(), v_cache.data_ptr(),
-        k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-        block_tables.shape[1], context_lens.data_ptr(), b, hq, hk, hd, bs, t, nb, float(softmax_scale), out.data_ptr(),
-        ors, workspace.data_ptr(), workspace.numel())
+        k_scales.data_ptr(), v_scales.data_ptr(), block_tables.data_ptr(), row, width, context_lens.data_ptr(), b, hq,
+        hk, hd, bs, t, nb, softmax_scale, out.data_ptr(), ors, workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -582,15 +601,18 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_n: int = 0
     [rows], top_tokens [rows, top_n] int64, top_logprobs [rows, top_n]), fp32."""
     _on_one_device(logits, token_ids)
     rows, vocab = logits.shape
-    assert logits.dtype in (torch.bfloat16, torch.float32) and (logits.stride(1) == 1 or vocab == 1)
-    assert token_ids.dtype == torch.int64 and token_ids.is_contiguous() and token_ids.shape == (rows,)
+    row, one = logits.stride()
+    dtype = logits.dtype
+    assert (dtype == _BF16 or dtype == _F32) and (one == 1 or vocab == 1)
+    assert token_ids.dtype == _I64 and token_ids.is_contiguous() and token_ids.shape == (rows,)
+    assert 0 <= top_n <= 32 and top_n <= vocab
     dev = logits.device
-    logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
-    entropies = torch.empty(rows, dtype=torch.float32, device=dev)
-    top_tokens = torch.empty(rows, top_n, dtype=torch.int64, device=dev)
-    top_logprobs = torch.empty(rows, top_n, dtype=torch.float32, device=dev)
+    logprobs = torch.empty(rows, dtype=_F32, device=dev)
+    entropies = torch.empty(rows, dtype=_F32, device=dev)
+    top_tokens = torch.empty((rows, top_n), dtype=_I64, device=dev)
+    top_logprobs = torch.empty((rows, top_n), dtype=_F32, device=dev)
     _launch(
-        "hl_token_logprobs", logits, logits.data_ptr(), 1 if logits.dtype == torch.float32 else 0, logits.stride(0) if
-        rows > 1 else vocab, rows, vocab, token_ids.data_ptr(), int(top_n), logprobs.data_ptr(), entropies.data_ptr(),
-        top_tokens.data_ptr(), top_logprobs.data_ptr())
+        "hl_token_logprobs", logits, logits.data_ptr(), 1 if dtype == _F32 else 0, row if rows > 1 else vocab, rows,
+        vocab, token_ids.data_ptr(), top_n, logprobs.data_ptr(), entropies.data_ptr(), top_tokens.data_ptr(),
+        top_logprobs.data_ptr())
     return logprobs, entropies, top_tokens, top_logprobs
