@@ -263,31 +263,34 @@ __device__ __noinline__ Merged merge_parts(const float2* __restrict__ part_ml, c
   return Merged{m, l, o};
 }
 
-// One sequence's `count` <= 16 parts of all G heads, merged in order and written to `out` by one warp:
-// four parts of four heads are in flight together.
+// One sequence's `count` <= 16 parts of all G heads, merged in order and written to `out` by one warp,
+// GC heads at a time with 16 loads a lane in flight.
+template <int GC>
 __device__ __noinline__ void merge_and_write(const float2* __restrict__ part_ml, const float* __restrict__ part_o,
                                              int count, int first, int rest, int stride, int group,
                                              __nv_bfloat16* __restrict__ out, int lane) {
-  for (int g0 = 0; g0 < group; g0 += 4) {
-    // Lane: part lane % 16, heads g0 + 2 (lane / 16) and the next.
-    const int i = lane & 15, gl = g0 + 2 * (lane >> 4);
-    float w[2], l[2];
+  constexpr int kParts = 16 / GC, kPairs = (GC + 1) / 2;
+  for (int g0 = 0; g0 < group; g0 += GC) {
+    // Lane: part lane % 16, heads g0 + kPairs (lane / 16) and the next.
+    const int i = lane & 15, gl = kPairs * (lane >> 4);
+    float w[kPairs], l[kPairs];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float2 ml = i < count && gl + x < group ? __ldcg(part_ml + (i == 0 ? first : rest + i * stride) + gl + x)
-                                                    : make_float2(-INFINITY, 0.f);
+    for (int x = 0; x < kPairs; ++x) {
+      const float2 ml = i < count && gl + x < GC && g0 + gl + x < group
+                            ? __ldcg(part_ml + (i == 0 ? first : rest + i * stride) + g0 + gl + x)
+                            : make_float2(-INFINITY, 0.f);
       w[x] = ml.x;
       l[x] = ml.y;
     }
-    float4 o[4];
+    float4 o[GC];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = 0; i0 < count; i0 += 4) {
-      float4 v[4][4];
+    for (int g = 0; g < GC; ++g) o[g] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < count; i0 += kParts) {
+      float4 v[kParts][GC];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < kParts; ++k)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < GC; ++g)
           v[k][g] = i0 + k < count && g0 + g < group
                         ? __ldcg(reinterpret_cast<const float4*>(
                                      part_o + int64_t((i0 + k == 0 ? first : rest + (i0 + k) * stride) + g0 + g) * kBlockHeadDim) +
@@ -295,7 +298,7 @@ __device__ __noinline__ void merge_and_write(const float2* __restrict__ part_ml,
                         : make_float4(0.f, 0.f, 0.f, 0.f);
       if (i0 == 0) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < kPairs; ++x) {
           float m = w[x];
 #pragma unroll
           for (int k = 8; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
@@ -306,10 +309,11 @@ __device__ __noinline__ void merge_and_write(const float2* __restrict__ part_ml,
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kParts; ++k) {
+        if (i0 + k >= count) break;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float wk = __shfl_sync(0xffffffffu, w[g & 1], 16 * (g >> 1) + ((i0 + k) & 15));
+        for (int g = 0; g < GC; ++g) {
+          const float wk = __shfl_sync(0xffffffffu, w[g % kPairs], 16 * (g / kPairs) + i0 + k);
           o[g].x = fmaf(v[k][g].x, wk, o[g].x);
           o[g].y = fmaf(v[k][g].y, wk, o[g].y);
           o[g].z = fmaf(v[k][g].z, wk, o[g].z);
@@ -318,8 +322,8 @@ __device__ __noinline__ void merge_and_write(const float2* __restrict__ part_ml,
       }
     }
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float sum = __shfl_sync(0xffffffffu, l[g & 1], 16 * (g >> 1));
+    for (int g = 0; g < GC; ++g) {
+      const float sum = __shfl_sync(0xffffffffu, l[g % kPairs], 16 * (g / kPairs));
       if (g0 + g >= group) continue;
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const __nv_bfloat162 lo = __floats2bfloat162_rn(o[g].x * inv, o[g].y * inv);
@@ -409,7 +413,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
   const int h = blockIdx.x % p.num_kv_heads, block = blockIdx.x / p.num_kv_heads, base = block * kWarps;
   const int ranges = min(int(gridDim.x) / p.num_kv_heads * kWarps, (total + kMinUnits - 1) / kMinUnits);
   // Ranges of `share` units, the first `more` of them of one more.
-  const unsigned share = unsigned(total) / max(ranges, 1), more = unsigned(total) - share * ranges;
+  const unsigned share = unsigned(total) / unsigned(max(ranges, 1)), more = unsigned(total) - share * ranges;
   auto range_begin = [&](int r) { return int(r * share + min(unsigned(r), more)); };
   auto range_of = [&](unsigned u) {  // that unit u lies in
     const unsigned wide = more * (share + 1);
@@ -420,6 +424,17 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (prefix[mid] <= u) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  };
+
+  auto warp_sequence_of = [&](int u) {  // the same for one u, by the lanes of a warp together
+    int lo = 0, n = p.batch;
+    while (n > 1) {
+      const int step = (n + 31) / 32, at = lane * step;
+      const int k = __popc(__ballot_sync(0xffffffffu, at < n && prefix[min(lo + at, p.batch - 1)] <= u)) - 1;
+      lo += k * step;
+      n = min(step, n - k * step);
     }
     return lo;
   };
@@ -473,7 +488,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
   const int range = base + warp;
   int u = range < ranges ? range_begin(range) : 0;
   const int end = range < ranges ? range_begin(range + 1) : 0;
-  int b = u < end ? sequence_of(u) : 0;
+  int b = u < end ? warp_sequence_of(u) : 0;
 
   const int part_stride = 2 * p.num_kv_heads * p.group;  // from one range's (or block's) parts to the next's
   const int c = lane & 3, rr = lane >> 2;
@@ -723,8 +738,11 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
         if (__shfl_sync(0xffffffffu, done, 0)) {
           if (own) __threadfence_block(); else __threadfence();
           const int from = 2 * (first * p.num_kv_heads + h) * p.group;
-          merge_and_write(p.part_ml, p.part_o, parts, from + p.group, from, part_stride, p.group,
-                          p.out + b * p.out_stride + int64_t(h) * p.group * kBlockHeadDim, lane);
+          __nv_bfloat16* out = p.out + b * p.out_stride + int64_t(h) * p.group * kBlockHeadDim;
+          if (p.group <= 2)
+            merge_and_write<2>(p.part_ml, p.part_o, parts, from + p.group, from, part_stride, p.group, out, lane);
+          else
+            merge_and_write<4>(p.part_ml, p.part_o, parts, from + p.group, from, part_stride, p.group, out, lane);
         }
       }
     }
@@ -737,7 +755,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
   for (int side = 0; side < 2; ++side) {
     const int border = range_begin(min(base + side * kWarps, ranges));
     if (border >= total) continue;
-    const int b = sequence_of(border);
+    const int b = warp_sequence_of(border);
     if (border <= prefix[b] + 1) continue;  // no tile of it lies in front
     const int first = range_of(prefix[b] + 1), last = range_of(prefix[b + 1] - 1);
     if (last - first < kDirectMerge || (side && first < base)) continue;
