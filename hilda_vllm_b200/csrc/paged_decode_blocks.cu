@@ -6,8 +6,10 @@
 //
 // Bound: HBM, 256 B of K and V per token and head.  One warp walks 32-token tiles of one KV head
 // with an online softmax; its K and V tiles arrive by TMA (128-byte swizzle) in a ring of three
-// 4 KiB slots of its own, issued by a ninth warp whose lane w serves warp w, so page lookups and
-// copies run ahead of the arithmetic and no consumer waits for another.
+// 4 KiB slots of its own, issued by an eighth warp whose lane w serves warp w, so page lookups and
+// copies run ahead of the arithmetic and no consumer waits for another.  Seven and one, twice an SM:
+// sixteen warps are four per scheduler with 128 registers each, with two more the tile loop spills
+// (256 contexts of 65-1087 tokens, GQA 2: 60 us against 64 us with eight and one).
 //
 // Both products run on m16n8k16 f16 MMAs with the cache as the A operand, the G query heads being
 // the 8 (16 for G > 8) columns: every cache byte is converted once (e4m3 -> f16, exact) and used by
@@ -23,7 +25,7 @@
 //
 // Work split: a thread block serves one KV head (neighbouring blocks the Hk heads of the same
 // tokens).  The tiles of all sequences, with one unit of cost more per sequence for its queries and
-// result, form a row that is cut into equal ranges, one per warp and eight per block.  A sequence
+// result, form a row that is cut into equal ranges, one per warp and seven per block.  A sequence
 // inside one warp's range is written out directly; one cut between warps leaves a part per warp in
 // the workspace (L2), and the warp that finishes last (a ticket, in shared memory where the block has
 // all parts) merges them in order, so results do not depend on the order of arrival.  A sequence of
@@ -40,7 +42,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxBatch = 4096;
-constexpr int kWarps = 8;
+constexpr int kWarps = 7;                          // that compute; one more loads
 constexpr int kTile = 32;                           // tokens of one tile
 constexpr int kTileBytes = kTile * kBlockHeadDim;   // one ring slot
 constexpr int kSlots = 3;
@@ -135,22 +137,20 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done;
 }
-// Copies one float and arrives on the barrier once it has landed.
-__device__ __forceinline__ void copy_float_arrive(float* dst, const float* src, uint64_t* bar) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // Token of MMA row r (mod 8).  K: lanes 0-7 of a shared load read rows 2i, 2i + 1, whose tokens
 // differ in bit 2; V: rows 0, 2, 4, 6 (or 1, 3, 5, 7) of two chunks, tokens that differ in bits 1-2.
 // The 128-byte swizzle XORs the 16-byte chunk with the token's low three bits: no conflicts.
 __device__ __forceinline__ int tile_row(int r) { return r ^ ((r & 1) << 2); }
 
+struct TileHead {
+  float scale;    // of the tile's group
+  int32_t valid;  // tokens it holds; 0: its page is outside the pool
+};
+
 struct Shared {
   uint8_t rows[kWarps][kSlots][kTileBytes];  // 1024-byte aligned slots
   uint64_t full[kWarps][kSlots], empty[kWarps][kSlots];
-  float scale[kWarps][kSlots];
-  int32_t valid[kWarps][kSlots];  // tokens the tile holds; 0: its page is outside the pool
+  TileHead head[kWarps][kSlots];
   int32_t warp_sum[kWarps + 1];
   int32_t last;             // broadcast of a ticket
   int32_t tickets[kWarps];  // sequences that begin in a warp's range and end in another's of the block
@@ -165,6 +165,7 @@ struct Loader {
   int n;           // tokens left in the sequence from this tile on
   int page_at, off, group_off, group;  // table index, token offset in the page, in its group; group in the page
   int page;        // block id, or -1
+  float ks, vs;    // the group's scales
 
   __device__ __forceinline__ void read_page(const BlockDecodeParams& p) {
     page = p.block_tables[b * p.bt_stride + page_at];
@@ -173,7 +174,12 @@ struct Loader {
       page = -1;
     }
   }
-  __device__ __forceinline__ void enter(const BlockDecodeParams& p, const int* prefix) {
+  __device__ __forceinline__ void read_scales(const BlockDecodeParams& p, int h) {
+    const int64_t at = page < 0 ? 0 : (int64_t(page) * (p.block_size / p.scale_block) + group) * p.num_kv_heads + h;
+    ks = __ldg(p.k_scales + at);
+    vs = __ldg(p.v_scales + at);
+  }
+  __device__ __forceinline__ void enter(const BlockDecodeParams& p, const int* prefix, int h) {
     if (u == prefix[b] && ++u >= end) return;  // the cost unit
     const int tok = (u - prefix[b] - 1) * kTile;
     n = min(p.context_lens[b], p.max_blocks * p.block_size) - tok;
@@ -183,39 +189,35 @@ struct Loader {
     group = off / p.scale_block;
     group_off = off - group * p.scale_block;
     read_page(p);
+    read_scales(p, h);
   }
   __device__ __forceinline__ void load(const BlockDecodeParams& p, Shared& sh, int w, int slot, int h, bool v) const {
     uint64_t* full = &sh.full[w][slot];
+    sh.head[w][slot] = TileHead{v ? vs : ks, page < 0 ? 0 : min(n, kTile)};
     if (page < 0) {
-      sh.valid[w][slot] = 0;
-      sh.scale[w][slot] = 0.f;
-      mbar_arrive(full);
       mbar_arrive(full);
       return;
     }
-    sh.valid[w][slot] = min(n, kTile);
     mbar_arrive_expect_tx(full, kTileBytes);
     tma_2d(sh.rows[w][slot], v ? &p.v_map : &p.k_map, h * kBlockHeadDim, page * p.block_size + off, full);
-    copy_float_arrive(&sh.scale[w][slot],
-                      (v ? p.v_scales : p.k_scales) +
-                          (int64_t(page) * (p.block_size / p.scale_block) + group) * p.num_kv_heads + h,
-                      full);
   }
-  __device__ __forceinline__ void next(const BlockDecodeParams& p, const int* prefix) {
+  __device__ __forceinline__ void next(const BlockDecodeParams& p, const int* prefix, int h) {
     if (++u >= end) return;
     if (u == b_end) {
       do ++b; while (prefix[b + 1] == u);  // sequences without tokens have no tiles
-      enter(p, prefix);
+      enter(p, prefix, h);
       return;
     }
     n -= kTile;
     off += kTile;
     group_off += kTile;
-    if (group_off == p.scale_block) group_off = 0, ++group;
+    if (group_off < p.scale_block) return;
+    group_off = 0, ++group;
     if (off == p.block_size) {
       off = 0, group = 0, ++page_at;
       read_page(p);
     }
+    read_scales(p, h);
   }
 };
 
@@ -381,7 +383,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < kWarps) sh.tickets[threadIdx.x] = 0;
   if (threadIdx.x < kWarps * kSlots) {
-    mbar_init(&sh.full[0][0] + threadIdx.x, 2);   // the tile's bytes and the scale
+    mbar_init(&sh.full[0][0] + threadIdx.x, 1);
     mbar_init(&sh.empty[0][0] + threadIdx.x, 1);
     fence_mbar_init();
   }
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
       ld.u = range_begin(range);
       ld.end = range_begin(range + 1);
       ld.b = sequence_of(ld.u);
-      ld.enter(p, prefix);
+      ld.enter(p, prefix, h);
     }
     int slot = 0, round = 0, idle = 0;
     bool v = false;
@@ -456,7 +458,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
       if (ld.u < ld.end) {
         if (mbar_test(&sh.empty[lane][slot], (round & 1) ^ 1)) {
           ld.load(p, sh, lane, slot, h, v);
-          if (v) ld.next(p, prefix);
+          if (v) ld.next(p, prefix, h);
           v = !v;
           if (++slot == kSlots) slot = 0, ++round;
           idle = 0;
@@ -593,8 +595,9 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
           }
         }
       }
-      const float ks = sh.scale[warp][slot];
-      const int valid = sh.valid[warp][slot];
+      const TileHead head = sh.head[warp][slot];
+      const float ks = head.scale;
+      const int valid = head.valid;
       advance();
 
       // ---- softmax
@@ -603,7 +606,13 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
         u = end;
         break;
       }
-      const float lv = __log2f(sh.scale[warp][slot]);
+      const float lv = __log2f(sh.head[warp][slot].scale);
+      const bool part = valid < kTile;  // the sequence's last tile: what lies behind is masked
+      if (part) {                       // and its values are zero, for 0 times what is there may be NaN
+        for (int i = valid * 32 + lane; i < kTile * 32; i += 32) reinterpret_cast<uint32_t*>(sh.rows[warp][slot])[i] = 0;
+        fence_proxy_async_smem();  // before the slot's next copy
+        __syncwarp();
+      }
       uint32_t pf[NT][2][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -618,7 +627,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
             for (int y = 0; y < 2; ++y) {
               float& v = s[mt][t][2 * y + x];
               v *= f;
-              if (valid < kTile && mt * 16 + y * 8 + tile_row(rr) >= valid) v = -INFINITY;
+              if (part && mt * 16 + y * 8 + tile_row(rr) >= valid) v = -INFINITY;
               mx = fmaxf(mx, v);
             }
 #pragma unroll
@@ -660,7 +669,6 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
         for (int k = 0; k < 4; ++k) {
           const int row = mt * 16 + (k >> 1) * 8 + tile_row(2 * c + (k & 1));
           v[k] = *reinterpret_cast<const uint4*>(sh.rows[warp][slot] + row * kBlockHeadDim + ((rr ^ (row & 7)) << 4));
-          if (valid < kTile && row >= valid) v[k] = make_uint4(0, 0, 0, 0);  // 0 x what lies there may be NaN
         }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
