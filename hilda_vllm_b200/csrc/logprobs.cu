@@ -64,22 +64,22 @@ __device__ __forceinline__ float2 pair(const uint4& v, int i, const float*) {
   return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
                 : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
 }
-// Largest and smallest logit of a batch of vectors (NaN ignored; NaN if there is nothing else).
+// Largest logit of a batch of vectors (NaN ignored; NaN if there is nothing else).
 template <int N>
-__device__ __forceinline__ float2 extremes(const uint4 (&v)[N], const __nv_bfloat16*) {
+__device__ __forceinline__ float largest(const uint4 (&v)[N], const __nv_bfloat16*) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v[0]);
-  __nv_bfloat162 hi = h[0], lo = h[0];
+  __nv_bfloat162 m = h[0];
 #pragma unroll
-  for (int i = 1; i < 4 * N; ++i) hi = __hmax2(hi, h[i]), lo = __hmin2(lo, h[i]);
-  return make_float2(fmaxf(__low2float(hi), __high2float(hi)), fminf(__low2float(lo), __high2float(lo)));
+  for (int i = 1; i < 4 * N; ++i) m = __hmax2(m, h[i]);
+  return fmaxf(__low2float(m), __high2float(m));
 }
 template <int N>
-__device__ __forceinline__ float2 extremes(const uint4 (&v)[N], const float*) {
+__device__ __forceinline__ float largest(const uint4 (&v)[N], const float*) {
   const float* f = reinterpret_cast<const float*>(&v[0]);
-  float hi = f[0], lo = f[0];
+  float m = f[0];
 #pragma unroll
-  for (int i = 1; i < 4 * N; ++i) hi = fmaxf(hi, f[i]), lo = fminf(lo, f[i]);
-  return make_float2(hi, lo);
+  for (int i = 1; i < 4 * N; ++i) m = fmaxf(m, f[i]);
+  return m;
 }
 
 // Whole numbers in the order of the logits: NaN lowest, then -inf ... +inf; -0 and +0 alike.  Never 0.
@@ -92,6 +92,8 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
   if (k == 1u) return NAN;
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
+
+constexpr uint32_t kMaskedKey = 0x007fffffu;  // of -inf; below it NaN only
 
 // Unique over a row: larger for a larger logit, and for a lower index among equals.  Never 0.
 __device__ __forceinline__ uint64_t entry_key(uint32_t key, int i) { return (uint64_t(key) << 32) | uint32_t(~i); }
@@ -185,15 +187,15 @@ template <int NT>
 struct LpShared {
   Softmax parts[(NT / 32)];
   Softmax sum;
-  uint32_t group_key[kGroups];
+  __align__(16) uint32_t group_key[kGroups];
   uint32_t threshold;
   int count, suspects;            // candidates; threads whose maximum reaches the threshold
   uint16_t suspect[NT];
   int scan[(NT / 32)];
   uint64_t best;
-  uint64_t candidates[kMaxCandidates];
+  __align__(16) uint64_t candidates[kMaxCandidates + 2];
   uint64_t top[kMaxTop];          // this block's, in order; 0 behind the last
-  uint64_t all[kMaxCluster * kMaxTop];
+  __align__(16) uint64_t all[kMaxCluster * kMaxTop + 2];
 };
 
 // This block's piece of a row.
@@ -210,7 +212,10 @@ struct Piece {
   }
   template <typename F>
   __device__ __forceinline__ void each_in(int v, F f) const {
-    const uint4 q = row.vector(v);
+    each_of(row.vector(v), v, f);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each_of(const uint4& q, int v, F f) const {  // q: vector v
 #pragma unroll
     for (int i = 0; i < Row<T>::kVec / 2; ++i) {
       const float2 x = pair(q, i, row.x);
@@ -228,24 +233,30 @@ struct Piece {
   }
 };
 
+// Before block_top, with a barrier in between.
+template <int NT>
+__device__ __forceinline__ void clear_top(LpShared<NT>& sh) {
+  const int tid = threadIdx.x;
+  if (tid < kGroups) sh.group_key[tid] = 0;
+  if (tid < kMaxTop) sh.top[tid] = 0;
+  if (tid == 0) sh.count = sh.suspects = 0;
+}
+
 // The top_n largest entries of the piece, in order, into sh.top.  mine: the key of this thread's
 // largest logit, 0 if it has none.
 template <typename T, int NT>
 __device__ void block_top(const Piece<T, NT>& piece, int top_n, uint32_t mine, LpShared<NT>& sh) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < kGroups) sh.group_key[tid] = 0;
-  if (tid < kMaxTop) sh.top[tid] = 0;
-  if (tid == 0) sh.count = sh.suspects = 0;
-  __syncthreads();
   atomicMax(&sh.group_key[tid % kGroups], mine);
   __syncthreads();
   if (tid < kGroups) {
     const uint32_t g = sh.group_key[tid];
     int rank = 0;
-#pragma unroll 16
-    for (int i = 0; i < kGroups; ++i) {
-      const uint32_t o = sh.group_key[i];
-      rank += o > g || (o == g && i < tid);
+#pragma unroll
+    for (int i = 0; i < kGroups; i += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&sh.group_key[i]);
+      rank += (o.x > g || (o.x == g && i < tid)) + (o.y > g || (o.y == g && i + 1 < tid)) +
+              (o.z > g || (o.z == g && i + 2 < tid)) + (o.w > g || (o.w == g && i + 3 < tid));
     }
     if (rank == top_n - 1) sh.threshold = g;
   }
@@ -264,10 +275,23 @@ __device__ void block_top(const Piece<T, NT>& piece, int top_n, uint32_t mine, L
       piece.each_single(tid, [&](float x, int i) { collect(x, i, least); });
     }
     __syncthreads();
-    const int each = (piece.end - piece.begin + NT - 1) / NT, n = sh.suspects * each;
-    for (int u = tid; u < n; u += NT) {
-      const int v = piece.begin + sh.suspect[u / each] + u % each * NT;
-      if (v < piece.end) piece.each_in(v, [&](float x, int i) { collect(x, i, least); });
+    // Warp w: suspects w, w + NT / 32, ..., two at a time; lane l: their vectors l, l + 32, ...
+    const float reach = key_logit(least);
+    const int n = sh.suspects, each = (piece.end - piece.begin + NT - 1) / NT;
+    for (int s0 = warp; s0 < n; s0 += 2 * (NT / 32)) {
+      const int s1 = s0 + NT / 32;
+      const int t0 = piece.begin + sh.suspect[s0], t1 = s1 < n ? piece.begin + sh.suspect[s1] : piece.end;
+      for (int k0 = lane; k0 < each; k0 += 64) {
+        int v[4] = {t0 + k0 * NT, t0 + (k0 + 32) * NT, t1 + k0 * NT, t1 + (k0 + 32) * NT};
+        uint4 q[4][1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (v[k] < piece.end) q[k][0] = piece.row.vector(v[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (v[k] < piece.end && (least <= kMaskedKey || largest(q[k], piece.row.x) >= reach))
+            piece.each_of(q[k][0], v[k], [&](float x, int i) { collect(x, i, least); });
+      }
     }
   };
   gather(threshold);
@@ -344,10 +368,16 @@ __device__ void block_top(const Piece<T, NT>& piece, int top_n, uint32_t mine, L
       return;
     }
   }
+  if (tid < 2) sh.candidates[count + tid] = 0;  // pairs below
+  __syncthreads();
   for (int i = tid; i < count; i += NT) {
     const uint64_t e = sh.candidates[i];
     int rank = 0;
-    for (int j = 0; j < count; ++j) rank += sh.candidates[j] > e;
+#pragma unroll 4
+    for (int j = 0; j < count; j += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.candidates[j]);
+      rank += (o.x > e) + (o.y > e);
+    }
     if (rank < top_n) sh.top[rank] = e;
   }
   __syncthreads();
@@ -367,6 +397,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
   const Row<T> row(logits + row_at * row_stride, vocab);
   const Piece<T, NT> piece{row, int(int64_t(row.vectors) * rank / blocks), int(int64_t(row.vectors) * (rank + 1) / blocks),
                        rank == 0, rank == blocks - 1};
+  if (top_n > 0) {
+    clear_top(sh);
+    __syncthreads();
+  }
   float asked = -INFINITY;  // the logit of the row's token
   if (rank == 0 && tid == 0) {
     const int64_t t = tokens[row_at];
@@ -394,16 +428,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
   };
   auto sum_batch = [&](uint4 (&q)[kUnroll], int v0) {
     if (v0 >= piece.end) return;
-    const float2 range = extremes(q, row.x);
-    thread_max = fmaxf(thread_max, range.x);
-    sm.raise_late(range.x);
-    if (!(range.y > -kHuge && sm.m < kHuge)) {  // masked or huge logits, or nothing but NaN: one by one
-      for (int k = 0; k < kUnroll; ++k) {
-        const int v = v0 + k * NT;
-        if (v < piece.end) piece.each_in(v, [&](float x, int) { sm.add(x); });
-      }
-      return;
-    }
+    const float top = largest(q, row.x);
+    thread_max = fmaxf(thread_max, top);
+    sm.raise_late(top);
     if (v0 + (kUnroll - 1) * NT >= piece.end) {  // behind the piece: -9e29, which adds nothing
       const uint32_t low = sizeof(T) == 2 ? 0xf135f135u : 0xf135be37u;
 #pragma unroll
@@ -418,7 +445,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
 #pragma unroll
       for (int i = 0; i < Row<T>::kVec / 2; ++i) {
         const float2 x = pair(q[k], i, row.x);
-        const uint64_t y = fma2(f32x2(x.x, x.y), scale, off);  // at least -3 kHuge: 2^y y is finite
+        const uint64_t y = fma2(f32x2(x.x, x.y), scale, off);
         const float2 yy = unpack(y);
         const uint64_t e = f32x2(ex2(yy.x), ex2(yy.y));
         z = add2(z, e);
@@ -426,8 +453,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
       }
     }
     const float2 zz = unpack(z), ss = unpack(s);
-    sm.z += zz.x + zz.y;
-    sm.s += ss.x + ss.y;
+    const float sum = ss.x + ss.y;
+    if (sum == sum && fabsf(sm.m) < kHuge) {
+      sm.z += zz.x + zz.y;
+      sm.s += sum;
+      return;
+    }
+    // Masked logits (2^-inf times -inf is NaN), huge ones or NaN: one by one.
+    for (int k = 0; k < kUnroll; ++k) {
+      const int v = v0 + k * NT;
+      if (v < piece.end) piece.each_in(v, [&](float x, int) { sm.add(x); });
+    }
   };
   uint4 even[kUnroll], odd[kUnroll];
   load(even, piece.begin + tid);
@@ -448,20 +484,28 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
   }
   if (blocks > 1) {
     cluster.sync();
-    const int n = blocks * top_n;
-    if (rank == 0) {
-      if (warp == 0) sm = warp_merge(*cluster.map_shared_rank(&sh.sum, lane % blocks), blocks);
-      if (tid < n) sh.all[tid] = cluster.map_shared_rank(sh.top, tid / top_n)[tid % top_n];
+    if (rank != 0) {
+      cluster.barrier_arrive();
+      cluster.barrier_wait();  // until the first block has read this one's shared memory
+      return;
     }
-    cluster.sync();  // the others' shared memory has been read
-    if (rank != 0) return;
+    const int n = blocks * top_n;
+    if (warp == 0) sm = warp_merge(*cluster.map_shared_rank(&sh.sum, lane % blocks), blocks);
+    if (tid < n) sh.all[tid] = cluster.map_shared_rank(sh.top, tid / top_n)[tid % top_n];
+    if (tid < (n & 1)) sh.all[n] = 0;  // pairs below
+    cluster.barrier_arrive();
+    __syncthreads();
     if (tid == 0) sh.sum = sm;
     if (tid < kMaxTop) sh.top[tid] = 0;
     __syncthreads();
     if (tid < n && sh.all[tid] != 0) {
       const uint64_t e = sh.all[tid];
       int r = 0;
-      for (int j = 0; j < n; ++j) r += sh.all[j] > e;
+#pragma unroll 8
+      for (int j = 0; j < n; j += 2) {
+        const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.all[j]);
+        r += (o.x > e) + (o.y > e);
+      }
       if (r < top_n) sh.top[r] = e;
     }
   }
@@ -484,6 +528,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
     top_tokens[row_at * top_n + tid] = int(~uint32_t(e));
     top_logprobs[row_at * top_n + tid] = logprob(key_logit(uint32_t(e >> 32)));
   }
+  if (blocks > 1) cluster.barrier_wait();  // completes the arrival above
 }
 
 template <typename T, int NT>
@@ -506,10 +551,18 @@ cudaError_t launch_logprobs_blocks(int blocks, const void* logits, int64_t row_s
 
 template <typename T, typename... Args>
 cudaError_t launch_logprobs(const void* logits, int64_t row_stride, int64_t rows, int vocab, Args... args) {
-  int blocks = 1;
-  while (blocks < kMaxCluster && rows * blocks < 148 && vocab / (2 * blocks) >= 512 * kUnroll * Row<T>::kVec / 2) blocks *= 2;
-  if (rows >= 4 * 148) return launch_logprobs_blocks<T, 256>(blocks, logits, row_stride, rows, vocab, args...);
-  return launch_logprobs_blocks<T, 512>(blocks, logits, row_stride, rows, vocab, args...);
+  // Up to a block of 512 threads for each half of an SM: those, and as many blocks a row as keep one an
+  // SM and a full batch of loads a thread (64 rows of 151936: two blocks 11.3 us, one 13.5, four 12.3).
+  // More rows: smaller blocks, whose barriers cost less, four an SM (512 rows: 35.6 us, with 512 threads
+  // 39.3), and eight for short rows (2048 rows of 1000: 15.3 us, with 256 threads 20.2).
+  if (rows <= 2 * 148) {
+    int blocks = 1;
+    while (blocks < kMaxCluster && 2 * rows * blocks <= 148 && vocab / (2 * blocks) >= 512 * kUnroll * Row<T>::kVec / 2)
+      blocks *= 2;
+    return launch_logprobs_blocks<T, 512>(blocks, logits, row_stride, rows, vocab, args...);
+  }
+  if (vocab >= 1024 * Row<T>::kVec) return launch_logprobs_blocks<T, 256>(1, logits, row_stride, rows, vocab, args...);
+  return launch_logprobs_blocks<T, 128>(1, logits, row_stride, rows, vocab, args...);
 }
 
 }  // namespace
