@@ -24,7 +24,7 @@ namespace {
 constexpr int kStoreThreads = 128;
 constexpr int kStoreWarps = kStoreThreads / 32;
 constexpr int kMaxWindow = 256;
-constexpr int kMaxSharedSeqs = 4096; // cu_seqlens_q of up to so many sequences is searched in shared memory
+constexpr int kMaxSharedSeqs = 4096;  // the lengths of up to so many sequences are searched in shared memory
 
 struct StoreBlocksParams {
   const __nv_bfloat16* x[2];  // key, value
@@ -54,8 +54,8 @@ struct GroupRun {
 };
 
 // The run that starts at row i; count 0 where i is inside a run or belongs to no sequence.
-// cu: the prefix sums, or nullptr for one row per sequence.
-__device__ GroupRun run_at(const StoreBlocksParams& p, const int32_t* cu, int64_t i) {
+// cu: the prefix sums, or nullptr for one row per sequence; context: the context lengths.
+__device__ GroupRun run_at(const StoreBlocksParams& p, const int32_t* cu, const int32_t* context, int64_t i) {
   GroupRun r{i, 0, 0, 0, 0};
   int64_t first = i, end = i + 1;  // rows of i's sequence
   int b = int(i);
@@ -71,7 +71,7 @@ __device__ GroupRun run_at(const StoreBlocksParams& p, const int32_t* cu, int64_
     end = cu[b + 1];
     if (first > i || first < 0) return r;
   }
-  const int64_t pos = int64_t(p.context_lens[b]) - (end - i);
+  const int64_t pos = int64_t(context[b]) - (end - i);
   if (pos < 0) return r;
   const unsigned at = unsigned(pos);  // < 2^31
   const unsigned j = at / unsigned(p.block_size), off = at - j * unsigned(p.block_size);
@@ -221,23 +221,27 @@ __device__ __forceinline__ void store_run(const StoreBlocksParams& p, const Grou
 
 template <int M, int L>
 __global__ void __launch_bounds__(kStoreThreads, L > 8 ? 3 : 8) store_kv_blocks_kernel(const __grid_constant__ StoreBlocksParams p) {
-  extern __shared__ int32_t cu_shared[];
+  extern __shared__ int32_t lens_shared[];  // [num_seqs + 1] cu, [num_seqs] context
   __shared__ GroupRun runs[kMaxWindow];
   __shared__ int found[kMaxWindow], num_found;
   __shared__ uint32_t team_max[kStoreWarps / M][M];
   const int item0 = blockIdx.y * p.items, items = min(p.items, 2 * p.num_kv_heads - item0);
   const int64_t begin = int64_t(blockIdx.x) * p.window;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int32_t* cu = p.cu;
+  const int32_t *cu = p.cu, *context = p.context_lens;
   if (cu && p.num_seqs <= kMaxSharedSeqs) {
-    for (int i = threadIdx.x; i <= p.num_seqs; i += kStoreThreads) cu_shared[i] = cu[i];
-    cu = cu_shared;
+    for (int i = threadIdx.x; i <= p.num_seqs; i += kStoreThreads) {
+      lens_shared[i] = cu[i];
+      if (i < p.num_seqs) lens_shared[p.num_seqs + 1 + i] = context[i];
+    }
+    cu = lens_shared;
+    context = lens_shared + p.num_seqs + 1;
   }
   const int window = int(min(int64_t(p.window), p.num_tokens - begin));
   if (threadIdx.x == 0) num_found = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < window; i += kStoreThreads) {
-    const GroupRun r = run_at(p, cu, begin + i);
+    const GroupRun r = run_at(p, cu, context, begin + i);
     runs[i] = r;
     if (r.count > 0) found[atomicAdd(&num_found, 1)] = i;
   }
@@ -253,18 +257,21 @@ void launch_store_blocks(StoreBlocksParams& p, int64_t window, int64_t items, cu
   p.window = int(window);
   p.items = int(items);
   const dim3 grid(unsigned((p.num_tokens + window - 1) / window), unsigned((2 * p.num_kv_heads + items - 1) / items));
-  const size_t shared = p.cu && p.num_seqs <= kMaxSharedSeqs ? (p.num_seqs + 1) * sizeof(int32_t) : 0;
+  const size_t shared = p.cu && p.num_seqs <= kMaxSharedSeqs ? (2 * p.num_seqs + 1) * sizeof(int32_t) : 0;
   store_kv_blocks_kernel<M, L><<<grid, kStoreThreads, shared, stream>>>(p);
 }
 
-// Windows of a group's rows, which start about one run each, and an item at least for each team of M
-// warps, more where that still makes twelve blocks an SM.
+// Windows of a group's rows, which start one run each and one more for every sequence that begins
+// there, and so many items that each team of M warps has one run of one item; more where that still
+// makes twelve blocks an SM.
 template <int M>
 void launch_store_prefill(StoreBlocksParams& p, cudaStream_t stream) {
   const int64_t window = p.scale_block < kMaxWindow ? p.scale_block : kMaxWindow, all = 2 * int64_t(p.num_kv_heads);
-  const int64_t teams = kStoreWarps / M, blocks = (p.num_tokens + window - 1) / window * all / (12 * 148);
-  const int64_t items = blocks > teams ? blocks / teams * teams : teams;
-  launch_store_blocks<M, 32>(p, window, items < all ? items : all, stream);
+  const int64_t teams = kStoreWarps / M, windows = (p.num_tokens + window - 1) / window, blocks = windows * all / (12 * 148);
+  const int64_t runs = windows + p.num_seqs;
+  int64_t items = blocks > teams ? blocks / teams * teams : (teams * windows + runs / 2) / runs;
+  items = items < 1 ? 1 : items > all ? all : items;
+  launch_store_blocks<M, 32>(p, window, items, stream);
 }
 
 }  // namespace

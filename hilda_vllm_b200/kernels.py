@@ -480,11 +480,10 @@ def extend_block_tables(block_tables: torch.Tensor, cached_lens: torch.Tensor | 
     assert cached_lens is None or (cached_lens.dtype == _I32 and cached_lens.is_contiguous()
                                    and cached_lens.shape == (b,))
     assert free_blocks.dtype == _I32 and free_blocks.is_contiguous() and free_blocks.dim() == 1
-    dev = block_tables.device
     # One allocation for the int32 results (slots first: 16-byte stores), one for the positions.
-    slots, cu_q, cu_k, context, status = torch.empty(
-        max_tokens + 3 * b + 4, dtype=_I32, device=dev).split_with_sizes((max_tokens, b + 1, b + 1, b, 2))
-    positions = torch.empty(max_tokens, dtype=_I64, device=dev)
+    slots, cu_q, cu_k, context, status = query_lens.new_empty(max_tokens + 3 * b + 4).split_with_sizes(
+        (max_tokens, b + 1, b + 1, b, 2))
+    positions = query_lens.new_empty(max_tokens, dtype=_I64)
     _launch(
         "hl_extend_block_tables", block_tables, None if cached_lens is None else cached_lens.data_ptr(),
         query_lens.data_ptr(), b, block_tables.data_ptr(), row, width, free_blocks.data_ptr(), free_blocks.numel(),
@@ -575,7 +574,7 @@ def paged_decode_fp8_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     assert context_lens.dtype == _I32 and context_lens.is_contiguous() and context_lens.numel() >= b
     ors = hq * hd
     if out is None:
-        out = torch.empty(shape, dtype=_BF16, device=q.device)
+        out = q.new_empty(shape)
     else:
         ors, ohs, oes = out.stride()
         assert out.dtype == _BF16 and out.shape == shape and (b == 0 or (oes == 1 and ohs == hd))
@@ -606,11 +605,10 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_n: int = 0
     assert (dtype == _BF16 or dtype == _F32) and (one == 1 or vocab == 1)
     assert token_ids.dtype == _I64 and token_ids.is_contiguous() and token_ids.shape == (rows,)
     assert 0 <= top_n <= 32 and top_n <= vocab
-    dev = logits.device
-    logprobs = torch.empty(rows, dtype=_F32, device=dev)
-    entropies = torch.empty(rows, dtype=_F32, device=dev)
-    top_tokens = torch.empty((rows, top_n), dtype=_I64, device=dev)
-    top_logprobs = torch.empty((rows, top_n), dtype=_F32, device=dev)
+    logprobs = logits.new_empty(rows, dtype=_F32)
+    entropies = logits.new_empty(rows, dtype=_F32)
+    top_tokens = token_ids.new_empty((rows, top_n))
+    top_logprobs = logits.new_empty((rows, top_n), dtype=_F32)
     _launch(
         "hl_token_logprobs", logits, logits.data_ptr(), 1 if dtype == _F32 else 0, row if rows > 1 else vocab, rows,
         vocab, token_ids.data_ptr(), top_n, logprobs.data_ptr(), entropies.data_ptr(), top_tokens.data_ptr(),
