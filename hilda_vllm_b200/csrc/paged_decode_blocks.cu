@@ -175,7 +175,9 @@ struct Loader {
     }
   }
   __device__ __forceinline__ void read_scales(const BlockDecodeParams& p, int h) {
-    const int64_t at = page < 0 ? 0 : (int64_t(page) * (p.block_size / p.scale_block) + group) * p.num_kv_heads + h;
+    ks = vs = 1.f;  // a tile without a page is masked; its scales have to be numbers
+    if (page < 0) return;
+    const int64_t at = (int64_t(page) * (p.block_size / p.scale_block) + group) * p.num_kv_heads + h;
     ks = __ldg(p.k_scales + at);
     vs = __ldg(p.v_scales + at);
   }

@@ -455,11 +455,12 @@ int hl_store_kv_fp8_blocks(const void* key, const void* value, int64_t key_row_s
 
 /* Decode attention over that cache: hl_paged_decode's arguments and result with the scales of the
  * groups in place of per-head ones (mini_vllm/layers/attention.py:134-141).  Scales may be any
- * finite fp32 values.  head_dim == 128, any Hk, Hq / Hk <= 16, batch <= 4096.  Tokens on a page
+ * finite fp32 values >= 0.  head_dim == 128, Hk <= 296, Hq / Hk <= 16, batch <= 4096.  Tokens on a page
  * outside [0, num_blocks) are left out and set bit 1 of the error word; contexts end at the table's
  * width; rows with context_lens <= 0 give zeros.  The workspace must be zero-filled once before
- * first use and is left ready for the next launch; launches that share it must not overlap.  Its
- * first word holds the error bits (hl_paged_decode_read_errors). */
+ * first use and is left ready for the next launch, of any shape it is large enough for; launches that
+ * share it must not overlap.  Its first word holds the error bits (hl_paged_decode_read_errors); after
+ * bit 0, a wait that gave up, zero-fill it again. */
 int64_t hl_paged_decode_fp8_blocks_workspace_size(int batch, int num_q_heads, int num_kv_heads);
 
 int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, const void* k_cache,

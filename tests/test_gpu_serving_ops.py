@@ -395,6 +395,19 @@ def test_decode_blocks_pages_outside_the_pool_and_narrow_tables():
     check_decode(q, kc, vc, ks, vs, tables, context, errors=2)
 
 
+def test_decode_blocks_page_outside_the_pool_with_nan_scales_elsewhere():
+    """A missing page is left out whatever the scales of pages that nobody asked for."""
+    q, kc, vc, ks, vs, tables, context = decode_case(15, 2, 4, 256, 64, [700, 300])
+    spare = (set(range(kc.shape[0])) - {p for row in tables for p in row}).pop()
+    for x in (kc, vc, ks, vs):
+        x.view(torch.uint8)[[0, spare]] = x.view(torch.uint8)[[spare, 0]]
+    tables = [[{0: spare, spare: 0}.get(p, p) for p in row] for row in tables]
+    assert all(0 not in row for row in tables)  # page 0 of the pool is the one that nobody asks for
+    ks[0] = vs[0] = math.nan
+    tables[0][1] = tables[1][0] = -1
+    check_decode(q, kc, vc, ks, vs, tables, context, errors=2)
+
+
 def test_decode_blocks_workspace_serves_calls_of_every_size_and_strided_rows():
     ws = kernels.make_block_decode_workspace(256, 32, 8, torch.device(DEV))
     for seed, (hk, group, context) in enumerate([(8, 4, [5000, 1, 77]), (8, 1, [400] * 200), (8, 3, [30000]), (8, 4, [64])]):
