@@ -19,7 +19,7 @@
 // through again, a warp for one thread's vectors, and the candidates are ranked by unique 64-bit
 // (logit, index) keys.  Where ties at the threshold are too many for the candidate buffer, those with
 // the lowest indices are taken in index order; where that many lie above it, rounds of block maxima.
-#include "hl_common.cuh"
+#include "dependent_launch.cuh"
 
 #include <cooperative_groups.h>
 
@@ -49,7 +49,7 @@ struct Row {
     vectors = (vocab - head) / kVec;
     tail = vocab - head - vectors * kVec;
   }
-  __device__ __forceinline__ uint4 vector(int v) const { return __ldg(reinterpret_cast<const uint4*>(x + head) + v); }
+  __device__ __forceinline__ uint4 vector(int v) const { return load16(x + head + int64_t(v) * kVec); }
 };
 
 __device__ __forceinline__ float load_logit(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -386,9 +386,9 @@ __device__ void block_top(const Piece<T, NT>& piece, int top_n, uint32_t mine, L
 // One cluster per row, each block a piece of it.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
-    const T* __restrict__ logits, int64_t row_stride, int vocab, const int64_t* __restrict__ tokens, int top_n,
-    float* __restrict__ logprobs, float* __restrict__ entropies, int64_t* __restrict__ top_tokens,
-    float* __restrict__ top_logprobs) {
+    const T* logits, int64_t row_stride, int vocab, const int64_t* tokens, int top_n,
+    float* logprobs, float* entropies, int64_t* top_tokens,
+    float* top_logprobs) {
   __shared__ LpShared<NT> sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
   const Row<T> row(logits + row_at * row_stride, vocab);
   const Piece<T, NT> piece{row, int(int64_t(row.vectors) * rank / blocks), int(int64_t(row.vectors) * (rank + 1) / blocks),
                        rank == 0, rank == blocks - 1};
+  dependent_start();
   if (top_n > 0) {
     clear_top(sh);
     __syncthreads();
@@ -535,18 +536,9 @@ template <typename T, int NT>
 cudaError_t launch_logprobs_blocks(int blocks, const void* logits, int64_t row_stride, int64_t rows, int vocab,
                                    const int64_t* tokens, int top_n, float* logprobs, float* entropies,
                                    int64_t* top_tokens, float* top_logprobs, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(rows * blocks));
-  cfg.blockDim = dim3(NT);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = blocks;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT>, static_cast<const T*>(logits), row_stride, vocab,
-                            tokens, top_n, logprobs, entropies, top_tokens, top_logprobs);
+  return launch_dependent(token_logprobs_kernel<T, NT>, dim3(unsigned(rows * blocks)), NT, 0, blocks, stream,
+                          static_cast<const T*>(logits), row_stride, vocab, tokens, top_n, logprobs, entropies,
+                          top_tokens, top_logprobs);
 }
 
 template <typename T, typename... Args>

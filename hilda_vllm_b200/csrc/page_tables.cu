@@ -13,7 +13,7 @@
 // slots are three dependent reads.  So every thread block scans all lengths itself (at most 4096, from
 // L2) instead of waiting for one that does, and no thread reads a table entry that another writes: a
 // token on a new page takes the page's id from the free list, as the thread that writes the row does.
-#include "hl_common.cuh"
+#include "dependent_launch.cuh"
 
 namespace hl {
 namespace {
@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_tables_kernel(const Tabl
   __shared__ Sums warp_sums[kTableThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
+  dependent_start();
   // ---- prefix sums over the sequences
   const int per = (p.num_seqs + kTableThreads - 1) / kTableThreads;
   const int b0 = min(int(threadIdx.x) * per, p.num_seqs), b1 = min(b0 + per, p.num_seqs);
@@ -216,7 +217,11 @@ extern "C" int hl_extend_block_tables(const int32_t* cached_lens, const int32_t*
   const int64_t by_rows = (num_seqs + kTableThreads / 32 - 1) / (kTableThreads / 32);
   const int64_t want = by_tokens > by_rows ? by_tokens : by_rows;
   const int blocks = want < 1 ? 1 : want > kMaxTableBlocks ? kMaxTableBlocks : int(want);
-  extend_tables_kernel<<<blocks, kTableThreads, (2 * num_seqs + 1) * sizeof(int32_t), static_cast<cudaStream_t>(stream)>>>(p);
-  HL_CHECK_LAUNCH("hl_extend_block_tables");
+  const cudaError_t e = launch_dependent(extend_tables_kernel, dim3(blocks), kTableThreads,
+                                         (2 * num_seqs + 1) * sizeof(int32_t), 1, static_cast<cudaStream_t>(stream), p);
+  if (e != cudaSuccess) {
+    set_error("hl_extend_block_tables: launch failed: %s", cudaGetErrorString(e));
+    return HL_ERR_CUDA;
+  }
   return HL_OK;
 }

@@ -31,6 +31,7 @@
 // all parts) merges them in order, so results do not depend on the order of arrival.  A sequence of
 // more than kDirectMerge parts is merged by whole blocks, to one part per block first, and more than
 // kFlatMerge of those in two levels, so that no warp reads many parts one after another.
+#include "dependent_launch.cuh"
 #include "kv_blocks.cuh"
 
 #include <cuda.h>
@@ -178,8 +179,8 @@ struct Loader {
     ks = vs = 1.f;  // a tile without a page is masked; its scales have to be numbers
     if (page < 0) return;
     const int64_t at = (int64_t(page) * (p.block_size / p.scale_block) + group) * p.num_kv_heads + h;
-    ks = __ldg(p.k_scales + at);
-    vs = __ldg(p.v_scales + at);
+    ks = p.k_scales[at];
+    vs = p.v_scales[at];
   }
   __device__ __forceinline__ void enter(const BlockDecodeParams& p, const int* prefix, int h) {
     if (u == prefix[b] && ++u >= end) return;  // the cost unit
@@ -231,7 +232,7 @@ struct Merged {
 // (m, l, o) of one head over `count` parts, the first at index `first`, the i-th at rest + i * stride,
 // summed in that order; a lane holds four dimensions.  All loads of up to 16 parts are in flight
 // together; a call of its own, so that they take no registers from the tile loop.
-__device__ __noinline__ Merged merge_parts(const float2* __restrict__ part_ml, const float* __restrict__ part_o,
+__device__ __noinline__ Merged merge_parts(const float2* part_ml, const float* part_o,
                                            int count, int first, int rest, int stride, int lane) {
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -270,9 +271,9 @@ __device__ __noinline__ Merged merge_parts(const float2* __restrict__ part_ml, c
 // One sequence's `count` <= 16 parts of all G heads, merged in order and written to `out` by one warp,
 // GC heads at a time with 16 loads a lane in flight.
 template <int GC>
-__device__ __noinline__ void merge_and_write(const float2* __restrict__ part_ml, const float* __restrict__ part_o,
+__device__ __noinline__ void merge_and_write(const float2* part_ml, const float* part_o,
                                              int count, int first, int rest, int stride, int group,
-                                             __nv_bfloat16* __restrict__ out, int lane) {
+                                             __nv_bfloat16* out, int lane) {
   constexpr int kParts = 16 / GC, kPairs = (GC + 1) / 2;
   for (int g0 = 0; g0 < group; g0 += GC) {
     // Lane: part lane % 16, heads g0 + kPairs (lane / 16) and the next.
@@ -389,6 +390,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
     mbar_init(&sh.empty[0][0] + threadIdx.x, 1);
     fence_mbar_init();
   }
+  dependent_start();
   // Units of each sequence and their prefix sums.
   {
     constexpr int kThreads = 32 * (kWarps + 1);
@@ -519,8 +521,8 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
         if (g < p.group) {
           const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.q_stride + (int64_t(h) * p.group + g) * kBlockHeadDim +
                                                             16 * (c + 4 * i));
-          v0 = __ldg(src);
-          v1 = __ldg(src + 1);
+          v0 = load16(src);
+          v1 = load16(src + 1);
         }
         w[i][0] = v0.x, w[i][1] = v0.y, w[i][2] = v0.z, w[i][3] = v0.w;
         w[i][4] = v1.x, w[i][5] = v1.y, w[i][6] = v1.z, w[i][7] = v1.w;
@@ -841,8 +843,11 @@ int launch_decode_blocks(const BlockDecodeParams& p, cudaStream_t s) {
   }
   int ctas = n * kPerSm < kMaxCtas ? n * kPerSm : kMaxCtas;
   if (ctas < p.num_kv_heads) ctas = p.num_kv_heads;
-  decode_blocks_kernel<NT><<<ctas, 32 * (kWarps + 1), kShared + 4 * (p.batch + 1), s>>>(p);
-  HL_CHECK_LAUNCH("hl_paged_decode_fp8_blocks");
+  e = launch_dependent(decode_blocks_kernel<NT>, dim3(ctas), 32 * (kWarps + 1), kShared + 4 * (p.batch + 1), 1, s, p);
+  if (e != cudaSuccess) {
+    set_error("hl_paged_decode_fp8_blocks: launch failed: %s", cudaGetErrorString(e));
+    return HL_ERR_CUDA;
+  }
   return HL_OK;
 }
 

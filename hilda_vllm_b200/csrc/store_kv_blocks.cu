@@ -16,6 +16,7 @@
 // for another but for the maximum of a longer run, which two or four warps share.  HBM bounds a
 // prefill (3 B an element): L = 32, twelve warps of 16 KB an SM.  A decode step is bound by its chain
 // of reads (sequence, table, scale): L = 8, more and smaller warps.
+#include "dependent_launch.cuh"
 #include "kv_blocks.cuh"
 
 namespace hl {
@@ -178,11 +179,11 @@ __device__ __forceinline__ void store_run(const StoreBlocksParams& p, const Grou
     const __nv_bfloat16* x = at.x + (i0 + row) * p.x_stride[kv] + e0;
     if (i0 + (sub + 1) * kHeldRows <= r.count) {
 #pragma unroll
-      for (int k = 0; k < L; ++k) v[k] = __ldg(reinterpret_cast<const uint4*>(x + k * step));
+      for (int k = 0; k < L; ++k) v[k] = load16(x + k * step);
     } else {
 #pragma unroll
       for (int k = 0; k < L; ++k)
-        v[k] = i0 + row + 2 * k < r.count ? __ldg(reinterpret_cast<const uint4*>(x + k * step)) : make_uint4(0, 0, 0, 0);
+        v[k] = i0 + row + 2 * k < r.count ? load16(x + k * step) : make_uint4(0, 0, 0, 0);
     }
   };
   auto run_max = [&](auto raise) {
@@ -228,6 +229,7 @@ __global__ void __launch_bounds__(kStoreThreads, L > 8 ? 3 : 8) store_kv_blocks_
   const int item0 = blockIdx.y * p.items, items = min(p.items, 2 * p.num_kv_heads - item0);
   const int64_t begin = int64_t(blockIdx.x) * p.window;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  dependent_start();
   const int32_t *cu = p.cu, *context = p.context_lens;
   if (cu && p.num_seqs <= kMaxSharedSeqs) {
     for (int i = threadIdx.x; i <= p.num_seqs; i += kStoreThreads) {
@@ -253,25 +255,25 @@ __global__ void __launch_bounds__(kStoreThreads, L > 8 ? 3 : 8) store_kv_blocks_
 }
 
 template <int M, int L>
-void launch_store_blocks(StoreBlocksParams& p, int64_t window, int64_t items, cudaStream_t stream) {
+cudaError_t launch_store_blocks(StoreBlocksParams& p, int64_t window, int64_t items, cudaStream_t stream) {
   p.window = int(window);
   p.items = int(items);
   const dim3 grid(unsigned((p.num_tokens + window - 1) / window), unsigned((2 * p.num_kv_heads + items - 1) / items));
   const size_t shared = p.cu && p.num_seqs <= kMaxSharedSeqs ? (2 * p.num_seqs + 1) * sizeof(int32_t) : 0;
-  store_kv_blocks_kernel<M, L><<<grid, kStoreThreads, shared, stream>>>(p);
+  return launch_dependent(store_kv_blocks_kernel<M, L>, grid, kStoreThreads, shared, 1, stream, p);
 }
 
 // Windows of a group's rows, which start one run each and one more for every sequence that begins
 // there, and so many items that each team of M warps has one run of one item; more where that still
 // makes twelve blocks an SM.
 template <int M>
-void launch_store_prefill(StoreBlocksParams& p, cudaStream_t stream) {
+cudaError_t launch_store_prefill(StoreBlocksParams& p, cudaStream_t stream) {
   const int64_t window = p.scale_block < kMaxWindow ? p.scale_block : kMaxWindow, all = 2 * int64_t(p.num_kv_heads);
   const int64_t teams = kStoreWarps / M, windows = (p.num_tokens + window - 1) / window, blocks = windows * all / (12 * 148);
   const int64_t runs = windows + p.num_seqs;
   int64_t items = blocks > teams ? blocks / teams * teams : (teams * windows + runs / 2) / runs;
   items = items < 1 ? 1 : items > all ? all : items;
-  launch_store_blocks<M, 32>(p, window, items, stream);
+  return launch_store_blocks<M, 32>(p, window, items, stream);
 }
 
 }  // namespace
@@ -327,14 +329,18 @@ extern "C" int hl_store_kv_fp8_blocks(const void* key, const void* value, int64_
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   // Fewer than four rows a sequence: a warp for each row and item (256 x 1 row, 8 heads: 6.6 us, with
   // the prefill kernel 12.3 us).
+  cudaError_t e;
   if (num_tokens < 4 * int64_t(num_seqs))
-    launch_store_blocks<1, 8>(p, kStoreWarps, 1, s);
+    e = launch_store_blocks<1, 8>(p, kStoreWarps, 1, s);
   else if (scale_block <= 64)
-    launch_store_prefill<1>(p, s);
+    e = launch_store_prefill<1>(p, s);
   else if (scale_block <= 128)
-    launch_store_prefill<2>(p, s);
+    e = launch_store_prefill<2>(p, s);
   else
-    launch_store_prefill<4>(p, s);
-  HL_CHECK_LAUNCH("hl_store_kv_fp8_blocks");
+    e = launch_store_prefill<4>(p, s);
+  if (e != cudaSuccess) {
+    set_error("hl_store_kv_fp8_blocks: launch failed: %s", cudaGetErrorString(e));
+    return HL_ERR_CUDA;
+  }
   return HL_OK;
 }

@@ -673,3 +673,42 @@ def test_two_streams_with_a_workspace_each():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_calls_queued_behind_each_other_keep_the_streams_order():
+    """Steps that each read what the one before wrote, without a wait between them, against the same
+    steps with one after every call."""
+    g = torch.Generator(device=DEV).manual_seed(50)
+    hq, hk, bs, t, nb, b, vocab, steps = 8, 2, 256, 64, 30, 9, 2000, 70
+    qkv = torch.randn(steps, b, hq + 2 * hk, D, generator=g, device=DEV).bfloat16() * torch.logspace(
+        -2, 2, steps, device=DEV).view(-1, 1, 1, 1).bfloat16()
+    head = torch.randn(hq * D, vocab, generator=g, device=DEV).bfloat16()
+    i32 = dict(dtype=torch.int32, device=DEV)
+    start = torch.tensor([0, 1, 62, 63, 64, 250, 255, 256, 400], **i32)
+    free = torch.arange(nb, **i32)
+
+    def run(wait):
+        pause = torch.cuda.synchronize if wait else lambda: None
+        caches = torch.zeros(2, nb, bs, hk, D, dtype=torch.uint8, device=DEV).view(E4M3)
+        scales = torch.zeros(2, nb, bs // t, hk, device=DEV)
+        tables, seen = torch.full((b, 3), -1, **i32), []
+        kernels.extend_block_tables(tables, None, torch.full((b,), 500, **i32), free, bs, 0)
+        ws, context = kernels.make_block_decode_workspace(b, hq, hk, torch.device(DEV)), start
+        for x in qkv:
+            plan = kernels.extend_block_tables(tables, context, torch.ones(b, **i32), free, bs, b)
+            pause()
+            context = plan["context_lens"]
+            kernels.store_kvcache_fp8_blocks(x[:, hq:hq + hk], x[:, hq + hk:], caches[0], caches[1], scales[0], scales[1],
+                                             tables, context, plan["cu_seqlens_q"])
+            pause()
+            out = kernels.paged_decode_fp8_blocks(x[:, :hq], caches[0], caches[1], scales[0], scales[1], tables, context,
+                                                  D ** -0.5, workspace=ws)
+            pause()
+            logits = out.view(b, -1) @ head
+            pause()
+            seen += [out, *kernels.token_logprobs(logits, plan["positions"] % vocab, 3), plan["slot_mapping"]]
+            pause()
+        return seen + [caches.view(torch.uint8), scales, tables]
+
+    for got, want in zip(run(False), run(True)):
+        assert torch.equal(got, want)
