@@ -481,14 +481,16 @@ def extend_block_tables(block_tables: torch.Tensor, cached_lens: torch.Tensor | 
                                    and cached_lens.shape == (b,))
     assert free_blocks.dtype == _I32 and free_blocks.is_contiguous() and free_blocks.dim() == 1
     # One allocation for the int32 results (slots first: 16-byte stores), one for the positions.
-    slots, cu_q, cu_k, context, status = query_lens.new_empty(max_tokens + 3 * b + 4).split_with_sizes(
-        (max_tokens, b + 1, b + 1, b, 2))
+    results = query_lens.new_empty(max_tokens + 3 * b + 4)
+    slots, cu_q, cu_k, context, status = torch.unsafe_split_with_sizes(results, (max_tokens, b + 1, b + 1, b, 2))
     positions = query_lens.new_empty(max_tokens, dtype=_I64)
+    at = results.data_ptr()
+    cu_at = at + 4 * max_tokens
     _launch(
         "hl_extend_block_tables", block_tables, None if cached_lens is None else cached_lens.data_ptr(),
         query_lens.data_ptr(), b, block_tables.data_ptr(), row, width, free_blocks.data_ptr(), free_blocks.numel(),
-        block_size, max_tokens, cu_q.data_ptr(), cu_k.data_ptr(), context.data_ptr(), positions.data_ptr(),
-        slots.data_ptr(), status.data_ptr())
+        block_size, max_tokens, cu_at, cu_at + 4 * b + 4, cu_at + 8 * b + 8, positions.data_ptr(), at,
+        cu_at + 12 * b + 8)
     return {"block_tables": block_tables, "cu_seqlens_q": cu_q, "cu_seqlens_k": cu_k, "context_lens": context,
             "positions": positions, "slot_mapping": slots, "status": status}
 
@@ -574,7 +576,7 @@ def paged_decode_fp8_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     assert context_lens.dtype == _I32 and context_lens.is_contiguous() and context_lens.numel() >= b
     ors = hq * hd
     if out is None:
-        out = q.new_empty(shape)
+        out = q.new_empty(b, hq, hd)
     else:
         ors, ohs, oes = out.stride()
         assert out.dtype == _BF16 and out.shape == shape and (b == 0 or (oes == 1 and ohs == hd))
@@ -607,8 +609,8 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_n: int = 0
     assert 0 <= top_n <= 32 and top_n <= vocab
     logprobs = logits.new_empty(rows, dtype=_F32)
     entropies = logits.new_empty(rows, dtype=_F32)
-    top_tokens = token_ids.new_empty((rows, top_n))
-    top_logprobs = logits.new_empty((rows, top_n), dtype=_F32)
+    top_tokens = token_ids.new_empty(rows, top_n)
+    top_logprobs = logits.new_empty(rows, top_n, dtype=_F32)
     _launch(
         "hl_token_logprobs", logits, logits.data_ptr(), 1 if dtype == _F32 else 0, row if rows > 1 else vocab, rows,
         vocab, token_ids.data_ptr(), top_n, logprobs.data_ptr(), entropies.data_ptr(), top_tokens.data_ptr(),
