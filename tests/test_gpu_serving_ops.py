@@ -183,7 +183,7 @@ def run_store(x, y, state, tables, context, cu):
     (8, 256, 64, [1] * 40, None), (8, 256, 64, [1, 0, 63, 64, 65, 255, 256, 257, 700], None),
     (1, 512, 256, [5, 600, 1, 0, 2000], None), (2, 256, 128, [130, 1, 1, 127], [126, 127, 128, 1]),
     (4, 768, 192, [400, 200], [191, 192]), (5, 256, 64, [3000], [0]), (3, 64, 64, [70, 1, 64], [10, 63, 64]),
-    (8, 256, 256, [1] * 300, None),
+    (8, 256, 256, [1] * 300, None), (32, 256, 64, [5500, 900], [0, 30]), (32, 256, 128, [9000, 2500], [0, 100]),
 ])
 @pytest.mark.parametrize("explicit", [True, False])
 def test_store_blocks_bit_exact(hk, bs, t, query, cached, explicit):
