@@ -26,10 +26,4 @@ __device__ __forceinline__ float ceil_pow2(float x) {
   return __uint_as_float(min(max(e, 1u), 253u) << 23);
 }
 
-// |x| where x is finite, else 0: infinities and NaN do not set a group's scale.
-__device__ __forceinline__ float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a < INFINITY ? a : 0.f;
-}
-
 }  // namespace hl

@@ -53,6 +53,7 @@ constexpr int kFlatMerge = 40;
 constexpr int kMinUnits = 2;                        // of a range: shorter ones cost more in merging
 constexpr int kMergeFan = 16;                       // parts of a first-level group
 constexpr int kMaxDevices = 64;
+constexpr int kGaveUp = 0x7fffffff;                 // in place of a unit: a wait ran out
 
 struct BlockDecodeParams {
   CUtensorMap k_map, v_map;  // [num_blocks * block_size rows][Hk * 128 B], boxes of 32 rows x 128 B
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
       // ---- S^T = K Q^T
       if (!mbar_wait(&sh.full[warp][slot], parity)) {
         if (lane == 0) atomicOr(p.errors, 1);
-        u = end;
+        u = kGaveUp;
         break;
       }
       float s[2][NT][4];
@@ -607,7 +608,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
       // ---- softmax
       if (!mbar_wait(&sh.full[warp][slot], parity)) {
         if (lane == 0) atomicOr(p.errors, 1);
-        u = end;
+        u = kGaveUp;
         break;
       }
       const float lv = __log2f(sh.head[warp][slot].scale);
@@ -759,6 +760,12 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
       }
     }
     do ++b; while (u < end && prefix[b + 1] == u);
+  }
+  if (u == kGaveUp) {  // copies that are still in flight (no more than the ring holds), with a limit each
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_wait(&sh.full[warp][slot], parity);
+      if (++slot == kSlots) slot = 0, parity ^= 1;
+    }
   }
 
   // ---- long sequences, which are cut at this block's first border (they came in), its last (they go
