@@ -11,8 +11,9 @@
 // are few rows (they meet in distributed shared memory), each thread keeps an online softmax of the
 // 16-byte vectors tid, tid + T, ... of its block's piece (T threads): Z = sum 2^y and S = sum 2^y y, where
 // y = x log2 e - R and R a whole number near its maximum, raised only when a logit exceeds it by far
-// (2^16): one FMA a logit, and parts of different R meet with exact powers of two.  The exponential
-// (one MUFU a logit) bounds it next.
+// (2^16): one FMA a logit, and parts of different R meet with exact powers of two.  The
+// instructions bound it next: 2048 rows of 151936 bf16 take 110 us, 0.87 of the copy rate, with one
+// exponential in four as a polynomial 119, for that saves MUFU work (two thirds busy) but issues more.
 // Alternatives come from the same pass.  The largest logit of each of 64 groups of threads is known;
 // the top_n-th largest of those is a threshold that at least top_n logits reach, and few more do
 // (some 24 for 20 of 151936 independent ones).  Only threads whose own maximum reaches it are looked
@@ -63,6 +64,24 @@ __device__ __forceinline__ float2 pair(const uint4& v, int i, const __nv_bfloat1
 __device__ __forceinline__ float2 pair(const uint4& v, int i, const float*) {
   return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
                 : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+}
+// A vector with nothing below -1e38, NaN kept: what a usual softmax adds up from a masked logit is 0 then,
+// not 0 times infinity (with a second look at the batches where that happened instead, rows with masked
+// logits took 1.6 to 4 times as long).  One instruction for two bf16 logits.
+__device__ __forceinline__ uint4 unmasked(uint4 v, const __nv_bfloat16*) {
+  auto cut = [](uint32_t w) {
+    const __nv_bfloat162 h = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&w), __float2bfloat162_rn(-1e38f));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  };
+  return make_uint4(cut(v.x), cut(v.y), cut(v.z), cut(v.w));
+}
+__device__ __forceinline__ uint4 unmasked(uint4 v, const float*) {
+  auto cut = [](uint32_t w) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0fFE967699;" : "=f"(r) : "f"(__uint_as_float(w)));
+    return __float_as_uint(r);
+  };
+  return make_uint4(cut(v.x), cut(v.y), cut(v.z), cut(v.w));
 }
 // Largest logit of a batch of vectors (NaN ignored; NaN if there is nothing else).
 template <int N>
@@ -262,9 +281,11 @@ __device__ void block_top(const Piece<T, NT>& piece, int top_n, uint32_t mine, L
   }
   __syncthreads();
   const uint32_t threshold = sh.threshold;
+  auto overflown = [&] { return *const_cast<volatile int*>(&sh.count) > kMaxCandidates; };  // then all are dropped
   auto collect = [&](float x, int i, uint32_t least) {
     const uint32_t key = logit_key(x);
     if (key < least) return;
+    if (overflown()) return;
     const int at = atomicAdd(&sh.count, 1);
     if (at < kMaxCandidates) sh.candidates[at] = entry_key(key, i);
   };
@@ -278,7 +299,7 @@ __device__ void block_top(const Piece<T, NT>& piece, int top_n, uint32_t mine, L
     // Warp w: suspects w, w + NT / 32, ..., two at a time; lane l: their vectors l, l + 32, ...
     const float reach = key_logit(least);
     const int n = sh.suspects, each = (piece.end - piece.begin + NT - 1) / NT;
-    for (int s0 = warp; s0 < n; s0 += 2 * (NT / 32)) {
+    for (int s0 = warp; s0 < n && !overflown(); s0 += 2 * (NT / 32)) {
       const int s1 = s0 + NT / 32;
       const int t0 = piece.begin + sh.suspect[s0], t1 = s1 < n ? piece.begin + sh.suspect[s1] : piece.end;
       for (int k0 = lane; k0 < each; k0 += 64) {
@@ -410,6 +431,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
   Softmax sm{-INFINITY, 0.f, 0.f};
   float thread_max = NAN;  // NaN: nothing else
   bool any = false;        // the thread has a logit
+  bool huge = false;       // its reference was too large for the sums below
   piece.each_single(tid, [&](float x, int) {
     sm.add(x);
     thread_max = fmaxf(thread_max, x);
@@ -438,14 +460,16 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
       for (int k = 1; k < kUnroll; ++k)
         if (v0 + k * NT >= piece.end) q[k] = make_uint4(low, low, low, low);
     }
-    const float minus = -origin(sm.m);
+    const float ref = sm.ref(), minus = -origin(ref);
+    huge |= !(fabsf(ref) < kHuge);
     const uint64_t off = f32x2(minus, minus), scale = f32x2(kLog2e, kLog2e);
     uint64_t z = 0, s = 0;  // (0.f, 0.f)
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) {
+      const uint4 u = unmasked(q[k], row.x);
 #pragma unroll
       for (int i = 0; i < Row<T>::kVec / 2; ++i) {
-        const float2 x = pair(q[k], i, row.x);
+        const float2 x = pair(u, i, row.x);
         const uint64_t y = fma2(f32x2(x.x, x.y), scale, off);
         const float2 yy = unpack(y);
         const uint64_t e = f32x2(ex2(yy.x), ex2(yy.y));
@@ -454,17 +478,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
       }
     }
     const float2 zz = unpack(z), ss = unpack(s);
-    const float sum = ss.x + ss.y;
-    if (sum == sum && fabsf(sm.m) < kHuge) {
-      sm.z += zz.x + zz.y;
-      sm.s += sum;
-      return;
-    }
-    // Masked logits (2^-inf times -inf is NaN), huge ones or NaN: one by one.
-    for (int k = 0; k < kUnroll; ++k) {
-      const int v = v0 + k * NT;
-      if (v < piece.end) piece.each_in(v, [&](float x, int) { sm.add(x); });
-    }
+    sm.z += zz.x + zz.y;
+    sm.s += ss.x + ss.y;
   };
   uint4 even[kUnroll], odd[kUnroll];
   load(even, piece.begin + tid);
@@ -473,6 +488,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
     sum_batch(even, v0);
     load(even, v0 + 2 * kUnroll * NT);
     sum_batch(odd, v0 + kUnroll * NT);
+  }
+  if (huge) {  // one by one (out of the loop, whose registers it would cost)
+    sm = Softmax{-INFINITY, 0.f, 0.f};
+    piece.each_of(tid, [&](float x, int) { sm.add(x); });
   }
   // ---- the block's sums
   sm = warp_merge(sm, 32);

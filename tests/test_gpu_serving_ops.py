@@ -487,7 +487,8 @@ def test_logprobs_random(rows, vocab, top, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("case", ["equal", "few_values", "masked", "one_left", "last", "spread", "zeros", "ascending", "outside"])
+@pytest.mark.parametrize("case", ["equal", "few_values", "masked", "one_left", "last", "spread", "zeros", "ascending", "huge_first",
+                                  "outside"])
 def test_logprobs_ties_masks_and_ranges(case, dtype):
     g = torch.Generator(device=DEV).manual_seed(9)
     rows, vocab, top = 6, 20011, 32
@@ -513,6 +514,9 @@ def test_logprobs_ties_masks_and_ranges(case, dtype):
         x *= 1e4
     elif case == "zeros":  # -0 and +0 are equal
         x = torch.where(torch.rand(x.shape, generator=g, device=DEV) < 0.5, 0.0, -0.0)
+    elif case == "huge_first":  # usual logits behind some that are far below them
+        x[:, :vocab // 2] = -2e30
+        tokens = tokens // 2 + vocab // 2
     elif case == "ascending":  # every next logit is a new maximum
         x = torch.arange(vocab, device=DEV).float().repeat(rows, 1) * 1e-2
     else:
