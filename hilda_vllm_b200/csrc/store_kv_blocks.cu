@@ -26,7 +26,7 @@ namespace {
 constexpr int kStoreThreads = 128;
 constexpr int kStoreWarps = kStoreThreads / 32;
 constexpr int kMaxWindow = 256;
-constexpr int kMaxSharedSeqs = 4096;  // the lengths of up to so many sequences are searched in shared memory
+constexpr int kSharedSeqs = 512;  // the lengths of up to so many sequences are searched in shared memory
 
 struct StoreBlocksParams {
   const __nv_bfloat16* x[2];  // key, value
@@ -56,24 +56,29 @@ struct GroupRun {
 };
 
 // The run that starts at row i; count 0 where i is inside a run or belongs to no sequence.
-// cu: the prefix sums, or nullptr for one row per sequence; context: the context lengths.
-__device__ GroupRun run_at(const StoreBlocksParams& p, const int32_t* cu, const int32_t* context, int64_t i) {
+// lens: the prefix sums (nullptr: one row per sequence) and context lengths of the sequences from
+// `base` on; i lies in one of lo .. hi or in none.
+struct Lengths {
+  const int32_t *cu, *context;
+  int base, lo, hi;
+};
+__device__ GroupRun run_at(const StoreBlocksParams& p, const Lengths& lens, int64_t i) {
   GroupRun r{i, 0, 0, 0, 0};
   int64_t first = i, end = i + 1;  // rows of i's sequence
   int b = int(i);
-  if (cu) {
-    int lo = 0, hi = p.num_seqs;
+  if (lens.cu) {
+    int lo = lens.lo, hi = lens.hi;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (cu[mid + 1] > i) hi = mid; else lo = mid + 1;
+      if (lens.cu[mid + 1 - lens.base] > i) hi = mid; else lo = mid + 1;
     }
     b = lo;
     if (b >= p.num_seqs) return r;
-    first = cu[b];
-    end = cu[b + 1];
-    if (first > i || first < 0) return r;
+    first = lens.cu[b - lens.base];
+    end = lens.cu[b + 1 - lens.base];
+    if (first > i || first < 0 || end <= i) return r;
   }
-  const int64_t pos = int64_t(context[b]) - (end - i);
+  const int64_t pos = int64_t(lens.context[b - lens.base]) - (end - i);
   if (pos < 0) return r;
   const unsigned at = unsigned(pos);  // < 2^31
   const unsigned j = at / unsigned(p.block_size), off = at - j * unsigned(p.block_size);
@@ -86,6 +91,20 @@ __device__ GroupRun run_at(const StoreBlocksParams& p, const int32_t* cu, const 
   r.group = page * (p.block_size / p.scale_block) + off / unsigned(p.scale_block);
   r.count = int(min(int64_t(p.scale_block) - held, min(end, p.num_tokens) - i));
   return r;
+}
+
+// The first sequence that ends behind row i (num_seqs: none), by the lanes of a warp together.
+__device__ int warp_sequence_of(const StoreBlocksParams& p, int64_t i, int lane) {
+  int lo = 0, n = p.num_seqs;  // it is one of lo .. lo + n
+  while (n > 0) {
+    const int step = (n + 31) / 32, at = min((lane + 1) * step, n) - 1;
+    const int k = __popc(__ballot_sync(0xffffffffu, p.cu[lo + at + 1] <= i));
+    if (k == 32) return lo + n;
+    const int next = min(k * step, n);
+    n = min((k + 1) * step, n) - 1 - next;
+    lo += next;
+  }
+  return lo;
 }
 
 // Running maximum of |x| over pairs of bf16 values: NaN is passed over, infinities are not.
@@ -223,7 +242,8 @@ __device__ __forceinline__ void store_run(const StoreBlocksParams& p, const Grou
 
 template <int M, int L>
 __global__ void __launch_bounds__(kStoreThreads, L > 16 ? 3 : L > 8 ? 4 : 8) store_kv_blocks_kernel(const __grid_constant__ StoreBlocksParams p) {
-  extern __shared__ int32_t lens_shared[];  // [num_seqs + 1] cu, [num_seqs] context
+  __shared__ int32_t lens_shared[2 * kSharedSeqs + 1];  // cu, context
+  __shared__ int bounds[2];
   __shared__ GroupRun runs[kMaxWindow];
   __shared__ int found[kMaxWindow], num_found;
   __shared__ uint32_t team_max[kStoreWarps / M][M];
@@ -231,20 +251,34 @@ __global__ void __launch_bounds__(kStoreThreads, L > 16 ? 3 : L > 8 ? 4 : 8) sto
   const int64_t begin = int64_t(blockIdx.x) * p.window;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   dependent_start();
-  const int32_t *cu = p.cu, *context = p.context_lens;
-  if (cu && p.num_seqs <= kMaxSharedSeqs) {
-    for (int i = threadIdx.x; i <= p.num_seqs; i += kStoreThreads) {
-      lens_shared[i] = cu[i];
-      if (i < p.num_seqs) lens_shared[p.num_seqs + 1 + i] = context[i];
-    }
-    cu = lens_shared;
-    context = lens_shared + p.num_seqs + 1;
-  }
   const int window = int(min(int64_t(p.window), p.num_tokens - begin));
+  Lengths lens{p.cu, p.context_lens, 0, 0, p.num_seqs};
+  if (p.cu) {
+    int seqs = p.num_seqs;
+    if (seqs > kSharedSeqs) {  // those of the window
+      if (warp < 2) {
+        const int b = warp_sequence_of(p, warp == 0 ? begin : begin + window - 1, lane);
+        if (lane == 0) bounds[warp] = b;
+      }
+      __syncthreads();
+      lens.lo = bounds[0];
+      lens.hi = bounds[1];
+      seqs = min(lens.hi + 1, p.num_seqs) - lens.lo;
+    }
+    if (seqs <= kSharedSeqs) {
+      for (int i = threadIdx.x; i <= seqs; i += kStoreThreads) {
+        lens_shared[i] = p.cu[lens.lo + i];
+        if (i < seqs) lens_shared[kSharedSeqs + 1 + i] = p.context_lens[lens.lo + i];
+      }
+      lens.cu = lens_shared;
+      lens.context = lens_shared + kSharedSeqs + 1;
+      lens.base = lens.lo;
+    }
+  }
   if (threadIdx.x == 0) num_found = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < window; i += kStoreThreads) {
-    const GroupRun r = run_at(p, cu, context, begin + i);
+    const GroupRun r = run_at(p, lens, begin + i);
     runs[i] = r;
     if (r.count > 0) found[atomicAdd(&num_found, 1)] = i;
   }
@@ -260,28 +294,39 @@ cudaError_t launch_store_blocks(StoreBlocksParams& p, int64_t window, int64_t it
   p.window = int(window);
   p.items = int(items);
   const dim3 grid(unsigned((p.num_tokens + window - 1) / window), unsigned((2 * p.num_kv_heads + items - 1) / items));
-  const size_t shared = p.cu && p.num_seqs <= kMaxSharedSeqs ? (2 * p.num_seqs + 1) * sizeof(int32_t) : 0;
-  return launch_dependent(store_kv_blocks_kernel<M, L>, grid, kStoreThreads, shared, 1, stream, p);
+  return launch_dependent(store_kv_blocks_kernel<M, L>, grid, kStoreThreads, 0, 1, stream, p);
 }
 
-// Windows of a group's rows, which start one run each and one more for every sequence that begins
-// there (of more groups where one has fewer items than the block has teams), and so many items that
-// each team of M warps has one run of one item; more where that still makes twelve blocks an SM.
-// Up to three rounds of runs on the GPU, more and smaller pieces even the SMs' shares out: twice the
-// warps a run, half the loads each (4096 tokens, 8 heads: 7.0 -> 5.9 us; 8195: 17.9 -> 16.5;
-// 64 sequences of 100 to 400: 31 -> 27; but 65536: 67 -> 70 to 74).
-template <int M>
-cudaError_t launch_store_prefill(StoreBlocksParams& p, cudaStream_t stream) {
-  const int64_t group = p.scale_block < kMaxWindow ? p.scale_block : kMaxWindow, all = 2 * int64_t(p.num_kv_heads);
-  const int64_t blocks = (p.num_tokens + group - 1) / group * all / (12 * 148);
-  if constexpr (M < 4)
-    if (blocks <= 2) return launch_store_blocks<2 * M, 16>(p, group, 2, stream);
-  const int64_t teams = kStoreWarps / M, wide = group * ((teams + all - 1) / all);
-  const int64_t window = wide < kMaxWindow ? wide : kMaxWindow, windows = (p.num_tokens + window - 1) / window;
-  const int64_t runs = windows + p.num_seqs;
-  int64_t items = blocks > teams ? blocks / teams * teams : (teams * windows + runs / 2) / runs;
-  items = items < 1 ? 1 : items > all ? all : items;
-  return launch_store_blocks<M, 32>(p, window, items, stream);
+// Blocks of kTeams teams of M warps: windows that start one run on average (more where a run has fewer
+// items than the block teams), each team one item of it, more where that still makes kTeams rounds of all
+// warps that the GPU holds at a time.
+template <int M, int L>
+cudaError_t launch_store(StoreBlocksParams& p, int64_t rows, int64_t runs, cudaStream_t stream) {
+  constexpr int kTeams = kStoreWarps / M, kPerSm = L > 16 ? 3 : L > 8 ? 4 : 8, kLeast = L == 16 && M == 4 ? 2 : kTeams;
+  const int64_t all = 2 * int64_t(p.num_kv_heads), rounds = runs * all / (kStoreWarps * kPerSm * 148);
+  int64_t items = rounds > kLeast ? rounds / kTeams * kTeams : kLeast;
+  items = items > all ? all : items;
+  const int64_t window = rows * (kTeams > items ? kTeams / items : 1);
+  return launch_store_blocks<M, L>(p, window < kMaxWindow ? window : kMaxWindow, items, stream);
+}
+
+// By the rows of an average run, as many registers and warps as hold it (128 sequences of 16 rows,
+// T 128: 6.7 us, with the registers for whole groups 34; 4096 decode tokens: 42 us, one item at a time
+// and all lengths in every block 124).  Up to three rounds of whole groups on the GPU, more and smaller
+// pieces even the SMs' shares out: twice the warps a run, half the loads each (4096 tokens, 8 heads:
+// 7.0 -> 5.9 us; 8195: 17.9 -> 16.5; 64 sequences of 100 to 400: 31 -> 27; but 65536: 67 -> 70 to 74).
+cudaError_t launch_store_by_runs(StoreBlocksParams& p, cudaStream_t stream) {
+  const int64_t group = p.scale_block, all = 2 * int64_t(p.num_kv_heads);
+  int64_t runs = (p.num_tokens + group - 1) / group + p.num_seqs;
+  runs = runs < p.num_tokens ? runs : p.num_tokens;
+  int64_t rows = (p.num_tokens + runs - 1) / runs;
+  if (10 * rows > 9 * group) rows = group;  // whole groups: a window each
+  const bool few = runs * all <= 3 * 12 * 148;
+  if (rows <= 16) return launch_store<1, 8>(p, rows, runs, stream);
+  if (rows <= 32) return launch_store<1, 16>(p, rows, runs, stream);
+  if (rows <= 64) return few ? launch_store<2, 16>(p, rows, runs, stream) : launch_store<1, 32>(p, rows, runs, stream);
+  if (rows <= 128) return few ? launch_store<4, 16>(p, rows, runs, stream) : launch_store<2, 32>(p, rows, runs, stream);
+  return launch_store<4, 32>(p, rows, runs, stream);
 }
 
 }  // namespace
@@ -335,17 +380,7 @@ extern "C" int hl_store_kv_fp8_blocks(const void* key, const void* value, int64_
   p.scale_block = scale_block;
   p.num_blocks = num_blocks;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // Fewer than four rows a sequence: a warp for each row and item (256 x 1 row, 8 heads: 5.4 us, with
-  // the prefill kernel 45 us).
-  cudaError_t e;
-  if (num_tokens < 4 * int64_t(num_seqs))
-    e = launch_store_blocks<1, 8>(p, kStoreWarps, 1, s);
-  else if (scale_block <= 64)
-    e = launch_store_prefill<1>(p, s);
-  else if (scale_block <= 128)
-    e = launch_store_prefill<2>(p, s);
-  else
-    e = launch_store_prefill<4>(p, s);
+  const cudaError_t e = launch_store_by_runs(p, s);
   if (e != cudaSuccess) {
     set_error("hl_store_kv_fp8_blocks: launch failed: %s", cudaGetErrorString(e));
     return HL_ERR_CUDA;

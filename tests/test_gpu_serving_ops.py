@@ -184,6 +184,9 @@ def run_store(x, y, state, tables, context, cu):
     (1, 512, 256, [5, 600, 1, 0, 2000], None), (2, 256, 128, [130, 1, 1, 127], [126, 127, 128, 1]),
     (4, 768, 192, [400, 200], [191, 192]), (5, 256, 64, [3000], [0]), (3, 64, 64, [70, 1, 64], [10, 63, 64]),
     (8, 256, 256, [1] * 300, None), (32, 256, 64, [5500, 900], [0, 30]), (32, 256, 128, [9000, 2500], [0, 100]),
+    # more sequences than are searched in shared memory, in all and between two rows of a window
+    (1, 64, 64, [1, 0, 2] * 400, None), (2, 64, 64, [3] + [0] * 1200 + [2, 0, 50], None), (1, 64, 64, [1] * 900, None),
+    (2, 128, 128, [20] * 30, None), (3, 256, 256, [40] * 20 + [250], None), (2, 256, 256, [100, 90, 120] * 5, None),
 ])
 @pytest.mark.parametrize("explicit", [True, False])
 def test_store_blocks_bit_exact(hk, bs, t, query, cached, explicit):
