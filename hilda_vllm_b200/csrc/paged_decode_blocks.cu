@@ -18,10 +18,15 @@
 // dimensions, a lane's pairs are two tokens' bytes of one dimension (byte permutes), P^T comes from
 // the S^T accumulators by an 8x8 transpose.  The MMA row r of a block of 8 is token tile_row(r), an
 // order in which every 16-byte shared load of K and of V is free of bank conflicts.
-// q is bf16 times an exact power of two per head, f16.  With lv = log2 vs of the tile, the weights
-// enter the second product as f16(2^(s + lv - M)), M the running maximum of s + lv, and the sum as
-// fp32 2^(s - m): scales of any range cost no precision, and the f16 rounding (2^-12) is relative to
-// the largest weighted value.  Maxima, sums and outputs are fp32; O is rescaled only when M grows.
+// q is bf16 times an exact power of two per head, f16 (its elements below 2^-25 of the largest lose
+// bits).  With lv = log2 vs of the tile, the weights enter the second product as
+// f16(2^(15 + s + lv - M)), M the running maximum of s + lv, and the sum as fp32 2^(s - m).  f16
+// because it is what the MMA takes beside the cache's exact f16 values; 2^15 because half of its range
+// would lie idle otherwise: a weight down to 2^-29 of the largest is rounded by 2^-12 of itself, a
+// smaller one by at most 2^-40 of the largest (without it 2^-14 and 2^-25, and what many light tokens
+// add beside one of weight 0.999 and little value was rounded away).  The exponentials are ex2.approx
+// (2^-22), lv is lg2.approx.  Maxima, sums and outputs are fp32; M is kept relative to m, so that large
+// scores do not cost its bits, and O is rescaled only when M grows.
 //
 // Work split: a thread block serves one KV head (neighbouring blocks the Hk heads of the same
 // tokens).  The tiles of all sequences, with one unit of cost more per sequence for its queries and
@@ -54,6 +59,7 @@ constexpr int kMinUnits = 2;                        // of a range: shorter ones 
 constexpr int kMergeFan = 16;                       // parts of a first-level group
 constexpr int kMaxDevices = 64;
 constexpr int kGaveUp = 0x7fffffff;                 // in place of a unit: a wait ran out
+constexpr float kWeightExp = 15.f;                  // the largest weight of the second product is 2^15
 
 struct BlockDecodeParams {
   CUtensorMap k_map, v_map;  // [num_blocks * block_size rows][Hk * 128 B], boxes of 32 rows x 128 B
@@ -120,6 +126,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The same with 65504 in place of infinity.
+__device__ __forceinline__ uint32_t pack_weights(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
 }
 __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -353,8 +365,9 @@ __device__ __forceinline__ void write_row(const BlockDecodeParams& p, int b, int
       make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
 }
 
-// 2^(mv - m), the factor from units of 2^mv to units of 2^m; 0 where nothing was summed.
-__device__ __forceinline__ float unit(float mv, float m) { return mv == -INFINITY ? 0.f : exp2f(mv - m); }
+// An accumulator of the second product from units of 2^(m + lead - 15) to units of 2^m / y (lead = -inf:
+// nothing was summed).  In this order neither step leaves the range of fp32 where the result does not.
+__device__ __forceinline__ float from_units(float o, float lead, float y) { return o * (exp2f(-kWeightExp) * y) * exp2f(lead); }
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
 
@@ -549,12 +562,12 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
       qs[t][0] = __shfl_sync(0xffffffffu, down, 8 * c) * p.scale_log2;
       qs[t][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4) * p.scale_log2;
     }
-    // m: running maximum of s, mv: of s + lv; o in units of 2^mv.
-    float m[NT][2], mv[NT][2], l[NT][2], o[NT][8][4];
+    // m: running maximum of s, lead: of s + lv, less m; o in units of 2^(m + lead - 15).
+    float m[NT][2], lead[NT][2], l[NT][2], o[NT][8][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) m[t][x] = mv[t][x] = -INFINITY, l[t][x] = 0.f;
+      for (int x = 0; x < 2; ++x) m[t][x] = lead[t][x] = -INFINITY, l[t][x] = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -637,22 +650,23 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
             }
 #pragma unroll
           for (int k = 4; k <= 16; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-          const float m2 = fmaxf(m[t][x], mx), mv2 = fmaxf(mv[t][x], mx + lv);
-          const float ref = m2 == -INFINITY ? 0.f : m2, refv = mv2 == -INFINITY ? 0.f : mv2;
-          grow[x] = ex2(mv[t][x] - refv);
+          const float m2 = fmaxf(m[t][x], mx), ref = m2 == -INFINITY ? 0.f : m2, back = m[t][x] - ref;
+          const float was = lead[t][x] + back, lead2 = fmaxf(was, (mx - ref) + lv);
+          const float up = lv - (lead2 == -INFINITY ? 0.f : lead2) + kWeightExp;
+          grow[x] = was == lead2 ? 1.f : ex2(was - lead2);
           float sum = 0.f;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               float& v = s[mt][t][2 * y + x];
-              sum += ex2(v - ref);
-              v = ex2(v + (lv - refv));
+              v -= ref;
+              sum += ex2(v);
+              v = ex2(v + up);
             }
-          l[t][x] = fmaf(l[t][x], ex2(m[t][x] - ref), sum);
-          if (mv2 == mv[t][x]) grow[x] = 1.f;
+          l[t][x] = fmaf(l[t][x], ex2(back), sum);
           m[t][x] = m2;
-          mv[t][x] = mv2;
+          lead[t][x] = lead2;
         }
         if (__any_sync(0xffffffffu, grow[0] != 1.f || grow[1] != 1.f)) {
 #pragma unroll
@@ -663,7 +677,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) pf[t][mt][y] = transpose8x8(pack_half2(s[mt][t][2 * y], s[mt][t][2 * y + 1]));
+          for (int y = 0; y < 2; ++y) pf[t][mt][y] = transpose8x8(pack_weights(s[mt][t][2 * y], s[mt][t][2 * y + 1]));
       }
 
       // ---- O^T += V^T P^T
@@ -706,11 +720,11 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
         for (int x = 0; x < 2; ++x) {
           const int g = t * 8 + 2 * c + x;
           if (g >= p.group) continue;
-          const float inv = l[t][x] == 0.f ? 0.f : unit(mv[t][x], m[t][x]) / l[t][x];
+          const float inv = l[t][x] == 0.f ? 0.f : 1.f / l[t][x], from = lead[t][x];
           uint32_t w[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const __nv_bfloat162 h2 = __floats2bfloat162_rn(o[t][j][x] * inv, o[t][j][2 + x] * inv);
+            const __nv_bfloat162 h2 = __floats2bfloat162_rn(from_units(o[t][j][x], from, inv), from_units(o[t][j][2 + x], from, inv));
             w[j] = *reinterpret_cast<const uint32_t*>(&h2);
           }
           uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.out_stride + (int64_t(h) * p.group + g) * kBlockHeadDim + 16 * rr);
@@ -725,11 +739,12 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), NT == 1 ? 2 : 1)
         for (int x = 0; x < 2; ++x) {
           const int g = t * 8 + 2 * c + x;
           if (g >= p.group) continue;
-          const float f = unit(mv[t][x], m[t][x]);
+          const float from = lead[t][x];
           float4* dst = reinterpret_cast<float4*>(p.part_o + int64_t(part + g) * kBlockHeadDim + 16 * rr);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            __stcg(dst + j, make_float4(o[t][2 * j][x] * f, o[t][2 * j][2 + x] * f, o[t][2 * j + 1][x] * f, o[t][2 * j + 1][2 + x] * f));
+            __stcg(dst + j, make_float4(from_units(o[t][2 * j][x], from, 1.f), from_units(o[t][2 * j][2 + x], from, 1.f),
+                                        from_units(o[t][2 * j + 1][x], from, 1.f), from_units(o[t][2 * j + 1][2 + x], from, 1.f)));
           if (rr == 0) __stcg(&p.part_ml[part + g], make_float2(m[t][x], l[t][x]));
         }
       // The last warp of a sequence of few parts merges them.

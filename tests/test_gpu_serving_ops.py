@@ -430,6 +430,33 @@ def test_decode_blocks_repeats_bit_for_bit():
         assert torch.equal(first, check_decode(q, kc, vc, ks, vs, tables, context, workspace=ws))
 
 
+@pytest.mark.parametrize("share", [0.999, 0.9999])
+@pytest.mark.parametrize("context,seqs", [(1000, 300), (8192, 296), (32768, 256)])
+@pytest.mark.parametrize("sink", ["zero", "small"])
+def test_decode_blocks_with_a_token_that_takes_nearly_all_the_weight(sink, context, seqs, share):
+    """Token 0 has `share` of the weight and values of (nearly) nothing, so that the small weights of the
+    others make up the output; as many sequences as let one warp walk most of one.  All of them read the
+    same pages, and half of the heads have values of one sign."""
+    hk, bs, t, scale = 8, 256, 64, D ** -0.5
+    g = torch.Generator(device=DEV).manual_seed(71)
+    nb = -(-context // bs)
+    kc = (torch.randn(nb, bs, hk, D, generator=g, device=DEV) * 90).clamp(-448, 448)
+    vc = (torch.randn(nb, bs, hk, D, generator=g, device=DEV) * 90).clamp(-448, 448)
+    vc[:, :, ::2] = vc[:, :, ::2].abs()
+    kc[..., 0] = 0
+    kc[0, 0] = 0
+    kc[0, 0, :, 0] = 256
+    vc[0, 0] = 0 if sink == "zero" else 2.0 ** -9
+    kc, vc = kc.to(E4M3), vc.to(E4M3)
+    ks = torch.exp2(torch.randint(-8, -5, (nb, bs // t, hk), generator=g, device=DEV).float())
+    vs = torch.exp2(torch.randint(-8, -5, (nb, bs // t, hk), generator=g, device=DEV).float())
+    q = torch.randn(seqs, hk, D, generator=g, device=DEV).bfloat16()
+    k = (kc.float() * ks.repeat_interleave(t, 1)[..., None]).view(-1, hk, D)[1:context]
+    others = torch.logsumexp(torch.einsum("bhd,nhd->bhn", q.float(), k) * scale, -1)
+    q[:, :, 0] = ((others + math.log(share / (1 - share))) / (scale * 256 * ks[0, 0])).bfloat16()
+    check_decode(q, kc, vc, ks, vs, [list(range(nb))] * seqs, [context] * seqs)
+
+
 def test_store_and_decode_blocks_behind_4_gib_of_cache():
     nb, bs, hk, t = 17000, 256, 8, 64  # 4.5 GB of keys, as much of values
     cache = torch.zeros(2, nb, bs, hk, D, dtype=torch.uint8, device=DEV).view(E4M3)
