@@ -11,9 +11,12 @@
 // are few rows (they meet in distributed shared memory), each thread keeps an online softmax of the
 // 16-byte vectors tid, tid + T, ... of its block's piece (T threads): Z = sum 2^y and S = sum 2^y y, where
 // y = x log2 e - R and R a whole number near its maximum, raised only when a logit exceeds it by far
-// (2^16): one FMA a logit, and parts of different R meet with exact powers of two.  The
-// instructions bound it next: 2048 rows of 151936 bf16 take 110 us, 0.87 of the copy rate, with one
-// exponential in four as a polynomial 119, for that saves MUFU work (two thirds busy) but issues more.
+// (2^16): one FMA a logit, and parts of different R meet with exact powers of two.  R stays 0 for logits
+// below -1e8, which add 0 then, as masked ones do whatever the value that masks them; only a piece with
+// nothing above -5e7, or with a logit above 1e8 (where R no longer resolves one), is summed again one by
+// one, relative to one of its logits.  The instructions bound it next: 2048 rows of 151936 bf16 take
+// 110 us, 0.87 of the copy rate, with one exponential in four as a polynomial 119, for that saves MUFU
+// work (two thirds busy) but issues more.
 // Alternatives come from the same pass.  The largest logit of each of 64 groups of threads is known;
 // the top_n-th largest of those is a threshold that at least top_n logits reach, and few more do
 // (some 24 for 20 of 151936 independent ones).  Only threads whose own maximum reaches it are looked
@@ -65,7 +68,7 @@ __device__ __forceinline__ float2 pair(const uint4& v, int i, const float*) {
   return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
                 : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
 }
-// A vector with nothing below -1e38, NaN kept: what a usual softmax adds up from a masked logit is 0 then,
+// A vector with nothing below -1e38, NaN kept: what the sums below add up from a masked logit is 0 then,
 // not 0 times infinity (with a second look at the batches where that happened instead, rows with masked
 // logits took 1.6 to 4 times as long).  One instruction for two bf16 logits.
 __device__ __forceinline__ uint4 unmasked(uint4 v, const __nv_bfloat16*) {
@@ -129,15 +132,25 @@ __device__ __forceinline__ float floor_exponent(float y) {
   return r;
 }
 
-// Logits from here on differ by more than any softmax resolves unless they are equal; log2 e times
-// them may overflow.
-constexpr float kHuge = 1e30f;
+// Below this size a reference m is taken as the whole number next to m log2 e, which fp32 holds to within
+// 8 there (from 1.5e9 on it misses by 128 and more, and its own 2^y would overflow).
+constexpr float kUsual = 1e8f;
+constexpr float kHuge = 1e30f;  // log2 e times it is far from overflow
 
 // y of a logit x for a part with reference m, one of its logits and no less than its maximum - 11:
-// x log2 e - ceil(m log2 e), or (x - m) log2 e for a huge m; -1000 at least.
+// x log2 e - ceil(m log2 e), or (x - m) log2 e for an m that is not usual; -1000 at least.
 __device__ __forceinline__ float origin(float m) { return ceilf(m * kLog2e); }
+__device__ __forceinline__ bool usual(float m) { return fabsf(m) < kUsual; }
 __device__ __forceinline__ float exponent(float x, float m) {
-  return floor_exponent(fabsf(m) < kHuge ? fmaf(x, kLog2e, -origin(m)) : (x - m) * kLog2e);
+  return floor_exponent(usual(m) ? fmaf(x, kLog2e, -origin(m)) : (x - m) * kLog2e);
+}
+// What y of reference `to` is less than y of reference m; kAll: of any size, not usual ones only.
+template <bool kAll>
+__device__ __forceinline__ float shift(float m, float to) {
+  if (!kAll) return floor_exponent(origin(m) - origin(to));
+  const float d = usual(m) ? (usual(to) ? origin(m) - origin(to) : fmaf(to, -kLog2e, origin(m)))
+                           : (usual(to) ? fmaf(m, kLog2e, -origin(to)) : (m - to) * kLog2e);
+  return floor_exponent(d);
 }
 
 // Online softmax: z = sum 2^y, s = sum 2^y y.
@@ -145,23 +158,25 @@ struct Softmax {
   float m, z, s;
 
   __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }
+  template <bool kAll>
   __device__ __forceinline__ void raise(float to) {
     if (!(to > m)) return;
     if (m != -INFINITY) {  // else z and s are 0, or NaN
-      const float d = fabsf(m) < kHuge && fabsf(to) < kHuge ? floor_exponent(origin(m) - origin(to))
-                                                            : floor_exponent((m - to) * kLog2e);
-      const float f = ex2(d);
+      const float d = shift<kAll>(m, to), f = ex2(d);
       s = f * fmaf(d, z, s);
       z *= f;
     }
     m = to;
   }
-  // The same where the reference would fall behind by more than 16 = 11 log2 e.
+  // The same where the reference would fall behind by more than 16 = 11 log2 e.  kAll = false: not to
+  // logits below -1e8; the sums are worthless once there was one above 1e8.
+  template <bool kAll>
   __device__ __forceinline__ void raise_late(float to) {
-    if (!(to <= m + 11.f)) raise(to);
+    if (!(to <= m + 11.f) && (kAll || to > -kUsual)) raise<kAll>(to);
   }
+  template <bool kAll>
   __device__ __forceinline__ void add(float x) {
-    raise_late(x);
+    raise_late<kAll>(x);
     const float y = exponent(x, ref()), e = ex2(y);
     z += e;
     s = fmaf(e, y, s);
@@ -172,7 +187,7 @@ struct Softmax {
 __device__ __forceinline__ Softmax warp_merge(Softmax a, int lanes) {
   float m = a.m;
   for (int o = lanes / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  a.raise(m);
+  a.raise<true>(m);
   for (int o = lanes / 2; o >= 1; o >>= 1) {
     a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
     a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
@@ -404,6 +419,15 @@ __device__ void block_top(const Piece<T, NT>& piece, int top_n, uint32_t mine, L
   __syncthreads();
 }
 
+// The sums of a piece whose logits are of any size, one by one; in every lane those of its warp.  A call,
+// for inside the kernel it costs the loop registers (2048 rows: 112.8 us, 109.8 with the call).
+template <typename T, int NT>
+__device__ __noinline__ Softmax add_one_by_one(const Piece<T, NT> piece) {
+  Softmax sm{-INFINITY, 0.f, 0.f};
+  piece.each_of(threadIdx.x, [&](float x, int) { sm.add<true>(x); });
+  return warp_merge(sm, 32);
+}
+
 // One cluster per row, each block a piece of it.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
@@ -431,9 +455,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
   Softmax sm{-INFINITY, 0.f, 0.f};
   float thread_max = NAN;  // NaN: nothing else
   bool any = false;        // the thread has a logit
-  bool huge = false;       // its reference was too large for the sums below
   piece.each_single(tid, [&](float x, int) {
-    sm.add(x);
+    sm.add<false>(x);
     thread_max = fmaxf(thread_max, x);
     any = true;
   });
@@ -453,15 +476,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
     if (v0 >= piece.end) return;
     const float top = largest(q, row.x);
     thread_max = fmaxf(thread_max, top);
-    sm.raise_late(top);
-    if (v0 + (kUnroll - 1) * NT >= piece.end) {  // behind the piece: -9e29, which adds nothing
+    sm.raise_late<false>(top);
+    if (v0 + (kUnroll - 1) * NT >= piece.end) {  // behind the piece: -9e29, which adds nothing to a usual reference
       const uint32_t low = sizeof(T) == 2 ? 0xf135f135u : 0xf135be37u;
 #pragma unroll
       for (int k = 1; k < kUnroll; ++k)
         if (v0 + k * NT >= piece.end) q[k] = make_uint4(low, low, low, low);
     }
     const float ref = sm.ref(), minus = -origin(ref);
-    huge |= !(fabsf(ref) < kHuge);
     const uint64_t off = f32x2(minus, minus), scale = f32x2(kLog2e, kLog2e);
     uint64_t z = 0, s = 0;  // (0.f, 0.f)
 #pragma unroll
@@ -489,15 +511,19 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
     load(even, v0 + 2 * kUnroll * NT);
     sum_batch(odd, v0 + kUnroll * NT);
   }
-  if (huge) {  // one by one (out of the loop, whose registers it would cost)
-    sm = Softmax{-INFINITY, 0.f, 0.f};
-    piece.each_of(tid, [&](float x, int) { sm.add(x); });
-  }
   // ---- the block's sums
   sm = warp_merge(sm, 32);
   if (lane == 0) sh.parts[warp] = sm;
   if (top_n > 0) block_top(piece, top_n, any ? logit_key(thread_max) : 0u, sh);
   __syncthreads();
+  const float part_m = sh.parts[lane % (NT / 32)].m;
+  if (!__any_sync(0xffffffffu, part_m > -0.5f * kUsual) || __any_sync(0xffffffffu, part_m >= kUsual)) {
+    // The same decision in every warp.  (2048 rows of -1e30 alone: 426 us, 110 of usual logits.)
+    sm = add_one_by_one(piece);
+    __syncthreads();
+    if (lane == 0) sh.parts[warp] = sm;
+    __syncthreads();
+  }
   if (warp == 0) {
     sm = warp_merge(sh.parts[lane % (NT / 32)], (NT / 32));
     if (lane == 0) sh.sum = sm;
@@ -536,7 +562,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
   const bool masked = sum.m == -INFINITY && sum.z == sum.z;  // every logit is -inf
   auto logprob = [&](float x) {
     if (x == -INFINITY && sum.z == sum.z) return -INFINITY;
-    if (x > -kHuge && fabsf(sum.m) < kHuge) return (fmaf(x, kLog2e, -origin(sum.m)) - log_z) * kLn2;
+    if (x > -kHuge && usual(sum.m)) return (fmaf(x, kLog2e, -origin(sum.m)) - log_z) * kLn2;
     return (x - sum.m) - log_z * kLn2;  // for a usual m: log z and its origin are below the rounding of x
   };
   if (tid == 0) {

@@ -607,6 +607,74 @@ def test_logprobs_strided_and_unaligned_rows(dtype):
         check_logprobs(wide[::2, lo:hi], torch.randint(0, hi - lo, (5,), generator=g, device=DEV), min(4, hi - lo))
 
 
+def check_logprobs_of_any_size(x, tokens, top):
+    """check_logprobs with a bound for logits of any size: the two 32-bit terms of a log probability, and
+    of an entropy, are each up to 16 ln 2 < 12 beyond what is left of them (sums are kept relative to a
+    logit of the row up to 11 below its maximum), with four roundings of 2^-24 of that and of x - m."""
+    lp, ent, ids, tlp = kernels.token_logprobs(x, tokens, top)
+    d = x.double()
+    m = d.amax(-1, keepdim=True)
+    y = torch.where(d == -math.inf, 0, d - m)
+    e = torch.where(d == -math.inf, 0, torch.exp(d - m))
+    z = e.sum(-1, keepdim=True)
+    ln_z, spread, second = torch.log(z), (e * y.abs()).sum(-1, keepdim=True) / z, (e * y * y).sum(-1, keepdim=True) / z
+    d_ln_z = (x.shape[1] / 1024 + 64) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -22 * spread
+    want = d - m - ln_z
+    tol = d_ln_z + 2.0 ** -22 * ((d - m).abs() + ln_z + 12)
+    at = tokens[:, None]
+    close(lp, want.gather(1, at).squeeze(1), tol.gather(1, at).squeeze(1))
+    close(ent, (ln_z + spread).squeeze(1), (d_ln_z * (1 + spread) + 2.0 ** -22 * (12 + second + spread + ln_z)).squeeze(1))
+    order = torch.sort(x.float() + 0.0, dim=-1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(ids, order)
+    close(tlp, want.gather(1, order), tol.gather(1, order))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mask", [-3e4, -6e7, -1.01e8, -1e9, -1e10, -1e12, -1e20, -9.5e29, -1e30, -1e38, "lowest"])
+def test_logprobs_of_rows_masked_with_a_finite_value(mask, dtype):
+    """Guided decoding: most of a row at one low value; whole threads, blocks of a cluster and the row's
+    ends see nothing else."""
+    value = torch.finfo(dtype).min if mask == "lowest" else mask
+    g = torch.Generator(device=DEV).manual_seed(60)
+    for rows, vocab, top in ((1, 151936, 5), (6, 151937, 32), (300, 9001, 3), (320, 1003, 20)):
+        x = (torch.randn(rows, vocab, generator=g, device=DEV) * 3).to(dtype)
+        keep = torch.rand(rows, vocab, generator=g, device=DEV) < torch.tensor([0.1, 0.001, 0.5], device=DEV)[torch.arange(rows, device=DEV) % 3][:, None]
+        keep[::2, :vocab // 2] = False
+        keep[:, 3 * vocab // 4] = True
+        tokens = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+        tokens[::2] = 3 * vocab // 4
+        check_logprobs_of_any_size(x.masked_fill(~keep, value), tokens, top)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("largest", [1e10, -1e10, 1e20, -1e20, 1e30, -9.5e29, -1e30, 3e38, -3e38, 5e7, -5e7, 2e8, -2e8])
+def test_logprobs_of_rows_whose_maximum_is_large(largest, dtype):
+    """Everything within a few steps of the type around one large value, the maximum a few times."""
+    g = torch.Generator(device=DEV).manual_seed(61)
+    for rows, vocab in ((2, 151936), (300, 3001)):
+        steps = torch.randint(-9, 1, (rows, vocab), generator=g, device=DEV)
+        steps[:, 7] = 0
+        x = (largest + steps * (abs(largest) * torch.finfo(dtype).eps)).to(dtype)
+        tokens = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+        tokens[0] = 7
+        check_logprobs_of_any_size(x, tokens, 20)
+        x[:, vocab // 3:] = -math.inf  # threads and blocks without a logit
+        tokens %= vocab // 3
+        check_logprobs_of_any_size(x, tokens, 20)
+
+
+@pytest.mark.parametrize("middle", [-1e8, 1e8, -5e7, 5e7])
+def test_logprobs_where_the_forms_of_the_exponent_meet(middle):
+    """fp32 logits a few of their steps (4 or 8) apart on both sides of the sizes where a reference
+    changes its form, sorted so that some threads see one side only."""
+    g = torch.Generator(device=DEV).manual_seed(62)
+    for rows, vocab in ((1, 151936), (40, 20011), (300, 1500)):
+        x = (middle + 8.0 * torch.randint(-9, 9, (rows, vocab), generator=g, device=DEV)).float()
+        x[:, vocab // 2:] = x[:, vocab // 2:].sort(-1).values
+        x[::2] = x[::2].flip(1)
+        check_logprobs_of_any_size(x, torch.randint(0, vocab, (rows,), generator=g, device=DEV), 8)
+
+
 def test_logprobs_rows_behind_4_gib():
     x = torch.zeros(9000, 262144, dtype=torch.bfloat16, device=DEV)
     x[:, 5] = 3
