@@ -560,14 +560,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(
   const Softmax sum = sh.sum;
   const float log_z = sum.z != sum.z ? sum.z : log2f(sum.z);
   const bool masked = sum.m == -INFINITY && sum.z == sum.z;  // every logit is -inf
+  // Both results are differences of numbers of up to 16, which round to the wrong side of 0 by up to 1e-6
+  // for a token that is nearly certain.  (Comparisons, which keep NaN.)
   auto logprob = [&](float x) {
     if (x == -INFINITY && sum.z == sum.z) return -INFINITY;
-    if (x > -kHuge && usual(sum.m)) return (fmaf(x, kLog2e, -origin(sum.m)) - log_z) * kLn2;
-    return (x - sum.m) - log_z * kLn2;  // for a usual m: log z and its origin are below the rounding of x
+    const float p = x > -kHuge && usual(sum.m) ? (fmaf(x, kLog2e, -origin(sum.m)) - log_z) * kLn2
+                                               : (x - sum.m) - log_z * kLn2;  // usual m: log z and its origin are below the rounding of x
+    return p > 0.f ? 0.f : p;
   };
   if (tid == 0) {
     logprobs[row_at] = logprob(asked);
-    entropies[row_at] = masked ? 0.f : (log_z - sum.s / sum.z) * kLn2;
+    const float entropy = (log_z - sum.s / sum.z) * kLn2;
+    entropies[row_at] = masked || entropy < 0.f ? 0.f : entropy;
   }
   if (tid < top_n) {
     const uint64_t e = sh.top[tid];

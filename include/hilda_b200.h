@@ -482,7 +482,8 @@ int hl_paged_decode_fp8_blocks(const void* q, int64_t q_row_stride, const void* 
  *   probable first, the lowest id first among equals (top_n = 0: both may be NULL).
  * A -inf logit is a masked token: probability 0.  A row with nothing else gives -inf, entropy 0 and
  * the lowest ids; a NaN or +inf in a row makes its log probabilities and entropy NaN, NaN logits
- * ranking last.
+ * ranking last.  Log probabilities are never above 0, entropies never below; a masked token may also
+ * carry a large finite value (its log probability is then that much below the others).
  * ---------------------------------------------------------------------------------- */
 int hl_token_logprobs(const void* logits, int logits_fp32, int64_t row_stride, int64_t rows, int vocab,
                       const int64_t* token_ids, int top_n, float* logprobs, float* entropies,

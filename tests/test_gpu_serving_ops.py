@@ -675,6 +675,19 @@ def test_logprobs_where_the_forms_of_the_exponent_meet(middle):
         check_logprobs_of_any_size(x, torch.randint(0, vocab, (rows,), generator=g, device=DEV), 8)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logprobs_are_never_positive_and_entropies_never_negative(dtype):
+    """Confident rows, whose own token is nearly certain."""
+    g = torch.Generator(device=DEV).manual_seed(63)
+    for rows, vocab in ((256, 20011), (1000, 3001), (2, 151936)):
+        x = (torch.randn(rows, vocab, generator=g, device=DEV) * 2.5).to(dtype)
+        tokens = torch.randint(0, vocab, (rows,), generator=g, device=DEV)
+        x.scatter_(1, tokens[:, None], (20 + 25 * torch.rand(rows, 1, generator=g, device=DEV)).to(dtype))
+        lp, ent, ids, tlp = kernels.token_logprobs(x, tokens, 3)
+        assert bool((lp <= 0).all()) and bool((tlp <= 0).all()) and bool((ent >= 0).all())
+        check_logprobs_of_any_size(x, tokens, 3)
+
+
 def test_logprobs_rows_behind_4_gib():
     x = torch.zeros(9000, 262144, dtype=torch.bfloat16, device=DEV)
     x[:, 5] = 3
