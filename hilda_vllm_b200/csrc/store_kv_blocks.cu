@@ -172,6 +172,7 @@ struct RunPlace {
 __device__ __forceinline__ float new_scale(uint32_t amax_bits, bool held, float old, float& ratio) {
   float s = scale_for(__uint_as_float(amax_bits << 16));
   ratio = 1.f;
+  if (held && old == 0.f) ratio = 0.f;  // they stand for 0, and have to under the new scale
   if (held && old > 0.f && old < INFINITY) {
     s = fmaxf(s, ceil_pow2(old));
     ratio = __fdiv_rn(old, s);

@@ -230,6 +230,31 @@ def test_store_blocks_token_by_token_grows_the_scale():
         assert same_bytes(got, want)
 
 
+@pytest.mark.parametrize("hk,t,query,cached", [(2, 64, [1] * 9, None), (3, 128, [20, 1, 90, 128, 200], [5, 127, 64, 1, 0]),
+                                               (2, 256, [1, 100, 400], [255, 30, 256 + 7])])
+@pytest.mark.parametrize("old", [0.0, 2.0 ** -140, 2.0 ** -60, 2.0 ** 100])
+def test_store_blocks_appends_to_groups_of_any_scale(hk, t, query, cached, old):
+    """A caller's own scales, zero among them: scale := max(old, what the new rows need), earlier rows times
+    old / new."""
+    g = torch.Generator().manual_seed(64)
+    cached = torch.randint(1, t, (len(query),), generator=g).tolist() if cached is None else cached
+    context = [c + q for c, q in zip(cached, query)]
+    nb = sum(-(-c // 256) for c in context) + 1
+    tables, cu = pages(g, context, 256, nb, max(-(-c // 256) for c in context)), np.concatenate(([0], np.cumsum(query))).tolist()
+    kc, ks = pool(g, nb, 256, hk, t)
+    vc, vs = pool(g, nb, 256, hk, t)
+    ks.fill_(old)
+    vs.fill_(old)
+    x = (torch.randn(2, cu[-1], hk, D, generator=g) * torch.exp2(torch.randint(-9, 4, (2, cu[-1], hk, 1), generator=g).float())).bfloat16()
+    x[1] *= min(max(old, 1e-30), 1e30)  # values about as large as the scale, which then stays
+    state = [s.to(DEV) for s in (kc, vc, ks, vs)]
+    run_store(x[0].to(DEV), x[1].to(DEV), state, tables, context, cu)
+    store_ref(x[0], kc, ks, tables, context, cu)
+    store_ref(x[1], vc, vs, tables, context, cu)
+    for got, want in zip(state, (kc, vc, ks, vs)):
+        assert same_bytes(got, want)
+
+
 def test_store_blocks_extreme_values():
     """Zeros, the type's smallest and largest, infinities, NaN; the borders of 448 * 2^k."""
     g = torch.Generator().manual_seed(4)
