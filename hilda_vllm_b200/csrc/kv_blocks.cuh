@@ -18,12 +18,4 @@ __device__ __forceinline__ float scale_for(float amax) {
   return __uint_as_float(uint32_t(max(e, int(kMinScaleExp))) << 23);
 }
 
-// The smallest power of two >= x (x positive and finite; at most 2^126).  A scale this store wrote
-// is one already; a caller's own scale is rounded up to one when a row is added to its group.
-__device__ __forceinline__ float ceil_pow2(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const uint32_t e = (u >> 23) + ((u & 0x7fffffu) ? 1u : 0u);
-  return __uint_as_float(min(max(e, 1u), 253u) << 23);
-}
-
 }  // namespace hl

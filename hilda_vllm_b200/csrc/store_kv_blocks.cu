@@ -6,6 +6,8 @@
 // group's scale if it holds rows from before this call (0 otherwise):
 //   s = max(s_old, smallest power of two with a / s <= 448, 2^-100)
 //   rows from before: e4m3(q * s_old / s);   new rows: e4m3(x / s), saturating;   scale := s.
+// A scale of this store's own is a power of two, and x / s one exact bf16 product.  A caller's own may be
+// any; while it is the larger one, the new rows are divided in fp32.
 // Sequence b's rows cu[b] .. cu[b+1]-1 are its tokens context_lens[b] - n .. context_lens[b]-1, so
 // "rows from before" are the tokens of the group in front of its first new one, whatever the page
 // held for an earlier owner.
@@ -172,22 +174,24 @@ struct RunPlace {
 __device__ __forceinline__ float new_scale(uint32_t amax_bits, bool held, float old, float& ratio) {
   float s = scale_for(__uint_as_float(amax_bits << 16));
   ratio = 1.f;
-  if (held && old == 0.f) ratio = 0.f;  // they stand for 0, and have to under the new scale
-  if (held && old > 0.f && old < INFINITY) {
-    s = fmaxf(s, ceil_pow2(old));
+  if (held && old >= 0.f && old < INFINITY) {
+    s = fmaxf(s, old);
     ratio = __fdiv_rn(old, s);
   }
   return s;
 }
-// 1 / s of a power of two between 2^-100 and 2^126.
+// s is a power of two with a normal inverse (s >= 2^-100).
+__device__ __forceinline__ bool has_inverse(float s) { return (__float_as_uint(s) & 0x7fffffu) == 0 && s <= 0x1p126f; }
+// Its inverse.
 __device__ __forceinline__ __nv_bfloat162 inverse_pow2(float s) {
   return __float2bfloat162_rn(__uint_as_float((254u << 23) - __float_as_uint(s)));
 }
 
 // M warps, one run of one item: warp `sub` of them holds rows 2 L sub .. 2 L (sub + 1) - 1, two a load; of
-// a run that is longer than 2 L M rows the same of every 2 L M, which are then read twice.
+// a run that is longer than 2 L M rows the same of every 2 L M, which are then read twice.  False, with
+// nothing written, where the group keeps an old scale that has no exact inverse.
 template <int M, int L>
-__device__ __forceinline__ void store_run(const StoreBlocksParams& p, const GroupRun& r, int kv, int head, int sub,
+__device__ __forceinline__ bool store_run(const StoreBlocksParams& p, const GroupRun& r, int kv, int head, int sub,
                                           int team, int lane, uint32_t* team_max) {
   constexpr int kHeldRows = 2 * L;
   const RunPlace at(p, r, kv, head);
@@ -229,6 +233,7 @@ __device__ __forceinline__ void store_run(const StoreBlocksParams& p, const Grou
   if (amax >= 0x7f80u) amax = run_max([](__nv_bfloat162& m, uint4 x) { raise_finite(m, x); });
   float ratio;
   const float s = new_scale(amax, r.held > 0, old, ratio);
+  if (!has_inverse(s)) return false;  // s is the old one: what is written below but for the new rows stays
   const __nv_bfloat162 inverse = inverse_pow2(s);
   for (int i0 = 0; i0 < r.count; i0 += M * kHeldRows) {
     if (twice) load(i0);
@@ -239,6 +244,28 @@ __device__ __forceinline__ void store_run(const StoreBlocksParams& p, const Grou
   }
   if (ratio != 1.f) rescale_rows(at.out + e0, row_bytes, r.held, ratio, 2 * sub + (lane >> 4), 2 * M);
   if (sub == 0 && lane == 0) *at.scale = s;
+  return true;
+}
+
+// The rows of a run whose group keeps an old scale without an exact inverse, by M warps.  Apart from
+// store_run, whose loop would pay for the divisions with registers.
+template <int M>
+__device__ __forceinline__ void store_divided(const StoreBlocksParams& p, const GroupRun& r, int kv, int head, int sub, int lane) {
+  if (r.held == 0) return;
+  const RunPlace at(p, r, kv, head);
+  const float s = *at.scale;
+  if (has_inverse(s)) return;
+  const int e0 = (lane & 15) * 8;
+  const int64_t row_bytes = int64_t(p.num_kv_heads) * kBlockHeadDim;
+  for (int i = 2 * sub + (lane >> 4); i < r.count; i += 2 * M) {
+    const uint4 v = load16(at.x + i * p.x_stride[kv] + e0);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t q[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      q[t] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(bf16lo(w[t]), s), __fdiv_rn(bf16hi(w[t]), s)), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<uint2*>(at.out + (r.held + i) * row_bytes + e0) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+  }
 }
 
 template <int M, int L>
@@ -284,9 +311,19 @@ __global__ void __launch_bounds__(kStoreThreads, L > 16 ? 3 : L > 8 ? 4 : 8) sto
     if (r.count > 0) found[atomicAdd(&num_found, 1)] = i;
   }
   __syncthreads();
+  bool stored = true;  // the same in all warps of a team
   for (int i = warp / M; i < num_found * items; i += kStoreWarps / M) {
     const int item = item0 + i % items;
-    store_run<M, L>(p, runs[found[i / items]], item & 1, item >> 1, warp % M, warp / M, lane, team_max[warp / M]);
+    stored &= store_run<M, L>(p, runs[found[i / items]], item & 1, item >> 1, warp % M, warp / M, lane, team_max[warp / M]);
+  }
+  if (stored) return;
+  if constexpr (M > 1)  // the team's scales are written
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / M), "n"(32 * M) : "memory");
+  else
+    __syncwarp();
+  for (int i = warp / M; i < num_found * items; i += kStoreWarps / M) {
+    const int item = item0 + i % items;
+    store_divided<M>(p, runs[found[i / items]], item & 1, item >> 1, warp % M, lane);
   }
 }
 

@@ -441,7 +441,9 @@ int hl_extend_block_tables(const int32_t* cached_lens, const int32_t* query_lens
  * b (cu_seqlens_q = NULL: one row per sequence), their pages the entries of its block-table row.
  * Per group and head: scale := max(its scale if the group holds tokens from before this call, the
  * smallest power of two s with max|x| / s <= 448 over the new rows, 2^-100); tokens from before are
- * rescaled (round to nearest even) when it grows, new ones are e4m3(x / scale), saturating.
+ * rescaled (round to nearest even, by the fp32 quotient) when it grows, new ones are e4m3(x / scale),
+ * saturating.  Scales that this call writes are powers of two; one found there may be any finite value
+ * >= 0 and is then kept where it is the larger.
  * Infinities and NaN do not set a scale; they are stored as +-448 and NaN.  Rows with no position
  * >= 0, no table entry, or a page outside [0, num_blocks) are skipped, as are rows behind
  * cu_seqlens_q[num_seqs].  A page that is written to belongs to one sequence.

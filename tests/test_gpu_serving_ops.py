@@ -232,10 +232,10 @@ def test_store_blocks_token_by_token_grows_the_scale():
 
 @pytest.mark.parametrize("hk,t,query,cached", [(2, 64, [1] * 9, None), (3, 128, [20, 1, 90, 128, 200], [5, 127, 64, 1, 0]),
                                                (2, 256, [1, 100, 400], [255, 30, 256 + 7])])
-@pytest.mark.parametrize("old", [0.0, 2.0 ** -140, 2.0 ** -60, 2.0 ** 100])
+@pytest.mark.parametrize("old", [0.0, 2.0 ** -140, 2.0 ** -60, 2.0 ** 100, 0.3, 1e-39, 5e-31, 2.0 ** 127, 3e38, 7 * 2.0 ** -13])
 def test_store_blocks_appends_to_groups_of_any_scale(hk, t, query, cached, old):
-    """A caller's own scales, zero among them: scale := max(old, what the new rows need), earlier rows times
-    old / new."""
+    """A caller's own scales, zero, no powers of two, subnormal ones and the type's largest among them: scale :=
+    max(old, what the new rows need), earlier rows times old / new."""
     g = torch.Generator().manual_seed(64)
     cached = torch.randint(1, t, (len(query),), generator=g).tolist() if cached is None else cached
     context = [c + q for c, q in zip(cached, query)]
