@@ -198,6 +198,12 @@ __global__ void __launch_bounds__(kTableThreads) extend_tables_kernel(const Tabl
   }
 }
 
+// The bytes of two arrays meet (a pointer of an array without entries may be anything).
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && a_bytes > 0 && b_bytes > 0 && x < y + uintptr_t(b_bytes) && y < x + uintptr_t(a_bytes);
+}
+
 }  // namespace
 }  // namespace hl
 
@@ -220,6 +226,15 @@ extern "C" int hl_extend_block_tables(const int32_t* cached_lens, const int32_t*
                    (num_free == 0 || free_blocks) &&
                    (num_seqs == 0 || (query_lens && block_tables && context_lens)),
                "hl_extend_block_tables: null pointer");
+  // Every block reads the lengths and the free list for itself, so none may be overwritten meanwhile.
+  const int64_t seqs = 4 * int64_t(num_seqs);
+  const struct { const void* at; int64_t bytes; } inputs[] = {{cached_lens, seqs}, {query_lens, seqs}, {free_blocks, 4 * num_free}},
+      outputs[] = {{cu_seqlens_q, seqs + 4}, {cu_seqlens_k, seqs + 4}, {context_lens, seqs}, {status, 8},
+                   {positions, 8 * max_tokens}, {slot_mapping, 4 * max_tokens}};
+  for (const auto& in : inputs)
+    for (const auto& out : outputs)
+      HL_CHECK_ARG(!overlap(in.at, in.bytes, out.at, out.bytes),
+                   "hl_extend_block_tables: a result overlaps the lengths or the free list");
   const TableParams p{cached_lens, query_lens, num_seqs, block_tables, bt_stride, max_blocks, free_blocks, num_free,
                       block_size, max_tokens, cu_seqlens_q, cu_seqlens_k, context_lens, positions, slot_mapping,
                       status, aligned16(positions) && aligned16(slot_mapping)};

@@ -417,7 +417,8 @@ int hl_sample_filtered(const void* logits, int64_t row_stride, int rows, int voc
  * status [2]: pages taken from free_blocks, then HL_TABLES_* bits; where a bit is set the pages or
  * tokens that do not fit are left out (-1) and everything else is as described.  num_seqs <= 4096;
  * the totals, and every slot, must stay below 2^31 (a slot that does not gets -1).
- * cached_lens may be NULL (all 0).
+ * cached_lens may be NULL (all 0).  No result may overlap the lengths, the free list or another result
+ * (the first two are refused); to carry lengths on, copy context_lens to cached_lens behind the call.
  * ---------------------------------------------------------------------------------- */
 #define HL_TABLES_NO_PAGES 1         /* free_blocks is too short */
 #define HL_TABLES_TOO_NARROW 2       /* a sequence needs more than max_blocks pages */

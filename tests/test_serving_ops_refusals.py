@@ -34,6 +34,18 @@ def test_tables_refusals(changed, text):
     call("hl_extend_block_tables", TABLES, changed, text=text)
 
 
+@pytest.mark.parametrize("result", ["cu_q", "cu_k", "ctx", "pos", "slots", "status"])
+@pytest.mark.parametrize("given,entries", [("cached", 4), ("query", 4), ("free", 9)])
+def test_tables_refuse_results_that_overwrite_what_is_read(result, given, entries):
+    """Among them context_lens == cached_lens: all blocks read the lengths while the first writes."""
+    apart = {k: ctypes.c_void_p(4096 * (i + 1)) for i, k in enumerate(("cached", "query", "tables", "free", "cu_q", "cu_k", "ctx", "pos",
+                                                                       "slots", "status"))}
+    sizes = dict(cu_q=20, cu_k=20, ctx=16, pos=80, slots=40, status=8)
+    first = apart[given].value
+    for at in (first, first + 4 * entries - 4, first - sizes[result] + 4):
+        call("hl_extend_block_tables", TABLES, {**apart, result: ctypes.c_void_p(at)}, text="overlaps")
+
+
 STORE = dict(key=P, value=P, krs=1024, vrs=1024, tokens=5, kc=P, vc=P, ks=P, vs=P, tables=P, stride=4, width=4, ctx=P, cu=P, seqs=3,
              hk=8, d=128, bs=256, t=64, nb=10)
 
