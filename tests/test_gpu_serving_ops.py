@@ -281,6 +281,26 @@ def test_store_blocks_extreme_values():
         assert same_bytes(got, want)
 
 
+@pytest.mark.parametrize("hk,bs,t,query", [(8, 256, 256, [6000] * 16), (5, 256, 64, [30000, 31000, 30500]), (5, 128, 128, [40000, 41000]),
+                                           (5, 64, 64, [1] * 4000)])
+def test_store_blocks_large_calls_bit_exact(hk, bs, t, query):
+    """As many rounds of the GPU as give a block several heads, the last block of a window fewer."""
+    g = torch.Generator(device=DEV).manual_seed(hk + bs + t)
+    cached = [(7 * i) % (bs - 1) for i in range(len(query))]
+    context = [c + n for c, n in zip(cached, query)]
+    nb, cu = sum(-(-c // bs) for c in context), np.concatenate(([0], np.cumsum(query))).tolist()
+    tables = pages(torch.Generator().manual_seed(1), context, bs, nb, max(-(-c // bs) for c in context))
+    x = torch.randn(2, cu[-1], hk, D, generator=g, device=DEV, dtype=torch.bfloat16)
+    x *= torch.exp2(torch.randint(-6, 6, (2, cu[-1], hk, 1), generator=g, device=DEV).float()).bfloat16()
+    state = [torch.randint(0, 127, (nb, bs, hk, D), generator=g, device=DEV, dtype=torch.uint8).view(E4M3) for _ in range(2)]
+    state += [torch.exp2(torch.randint(-9, -4, (nb, bs // t, hk), generator=g, device=DEV).float()) for _ in range(2)]
+    want = [s.cpu() for s in state]
+    run_store(x[0], x[1], state, tables, context, cu)
+    for i in range(2):
+        store_ref(x[i].cpu(), want[i], want[2 + i], tables, context, cu)
+        assert torch.equal(state[2 + i].cpu(), want[2 + i]) and same_bytes(state[i], want[i])
+
+
 def test_store_blocks_skips_what_has_no_place():
     """Padding rows (context 0), pages outside the pool, positions before 0 or behind the table."""
     g = torch.Generator().manual_seed(5)
@@ -445,6 +465,16 @@ def test_decode_blocks_workspace_serves_calls_of_every_size_and_strided_rows():
         out = torch.zeros(len(context), hk * group + 2, D, dtype=torch.bfloat16, device=DEV)
         check_decode(wide[:, 2:-4], kc, vc, ks, vs, tables, context, workspace=ws, out=out[:, 1:-1])
         assert not out[:, 0].any() and not out[:, -1].any()
+
+
+def test_decode_blocks_4096_sequences():
+    """The largest batch: short, partly empty contexts that share a few pages."""
+    q, kc, vc, ks, vs, tables, _ = decode_case(72, 2, 4, 256, 64, [500] * 8)
+    g = torch.Generator().manual_seed(73)
+    context = torch.randint(0, 400, (4096,), generator=g).tolist()
+    context[::5] = [0] * len(context[::5])
+    q = torch.randn(4096, 8, D, generator=g).bfloat16().to(DEV)
+    check_decode(q, kc, vc, ks, vs, [tables[i % 8] for i in range(4096)], context)
 
 
 def test_decode_blocks_repeats_bit_for_bit():
@@ -852,3 +882,58 @@ def test_calls_queued_behind_each_other_keep_the_streams_order():
 
     for got, want in zip(run(False), run(True)):
         assert torch.equal(got, want)
+
+
+def test_captured_behind_copies_fills_and_joined_branches():
+    """Graphs whose launches follow a memset, a copy or two branches of the capture, and two graphs that use
+    one workspace in turn."""
+    g = torch.Generator(device=DEV).manual_seed(74)
+    q, kc, vc, ks, vs, tables, context = decode_case(75, 4, 4, 256, 64, [3000, 1, 700, 0, 65])
+    i32 = dict(dtype=torch.int32, device=DEV)
+    tables, context = torch.tensor(tables, **i32), torch.tensor(context, **i32)
+    x = torch.randn(5, 2, 4, D, generator=g, device=DEV).bfloat16()
+    logits = torch.randn(5, 20011, generator=g, device=DEV).bfloat16()
+    tokens, free = torch.arange(5, device=DEV), torch.arange(50, **i32)
+    ws = kernels.make_block_decode_workspace(5, 16, 4, q.device)
+    start = [t.clone() for t in (kc.view(torch.uint8), vc.view(torch.uint8), ks, vs)]
+    state = (kc.view(torch.uint8), vc.view(torch.uint8), ks, vs)
+    ones = torch.ones(5, **i32)
+
+    def step(workspace, split):
+        main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+        table = torch.full_like(tables, -1)                      # a fill in front of the table kernel
+        plan = kernels.extend_block_tables(table, None, ones, free, 256, 8)
+        if split:
+            side.wait_stream(main)
+            with torch.cuda.stream(side):
+                lp = kernels.token_logprobs(logits, tokens, 4)
+            kernels.store_kvcache_fp8_blocks(x[:, 0], x[:, 1], kc, vc, ks, vs, tables, context)
+            main.wait_stream(side)                               # two branches in front of the attention
+        else:
+            kernels.store_kvcache_fp8_blocks(x[:, 0], x[:, 1], kc, vc, ks, vs, tables, context)
+            lp = kernels.token_logprobs(logits, tokens, 4)
+        out = kernels.paged_decode_fp8_blocks(q, kc, vc, ks, vs, tables, context, D ** -0.5, workspace=workspace)
+        copied = out.clone()                                     # a copy in front of the next call
+        return [plan["slot_mapping"], table, *lp, copied, *kernels.token_logprobs(copied.view(5, -1), tokens, 3)]
+
+    want = [t.clone() for t in step(ws, False)]
+    after = [t.clone() for t in state]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(None, True)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for workspace, split in ((ws, True), (ws, False), (None, True)):  # None: its fill is part of the graph
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(workspace, split)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for graph, out in graphs:
+            for t, s in zip(state, start):
+                t.copy_(s)
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+            assert all(torch.equal(a, b) for a, b in zip(state, after))
+    assert kernels.decode_errors(ws) == 0
