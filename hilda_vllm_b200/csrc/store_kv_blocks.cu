@@ -337,7 +337,9 @@ cudaError_t launch_store_blocks(StoreBlocksParams& p, int64_t window, int64_t it
 
 // Blocks of kTeams teams of M warps: windows that start one run on average (more where a run has fewer
 // items than the block teams), each team one item of it, more where that still makes kTeams rounds of all
-// warps that the GPU holds at a time.
+// warps that the GPU holds at a time.  A block of one team of light warps (L = 16, M = 4) takes two items at
+// least, for one does not pay for the lookup of its run (64 sequences of 250, 8 heads: 20.3 us, 22.8 with one
+// item; 16 of 500: 9.5 and 10.7; but 2 heads: 8.1 and 6.6).
 template <int M, int L>
 cudaError_t launch_store(StoreBlocksParams& p, int64_t rows, int64_t runs, cudaStream_t stream) {
   constexpr int kTeams = kStoreWarps / M, kPerSm = L > 16 ? 3 : L > 8 ? 4 : 8, kLeast = L == 16 && M == 4 ? 2 : kTeams;
