@@ -18,7 +18,7 @@
 // dimensions, a lane's pairs are two tokens' bytes of one dimension (byte permutes), P^T comes from
 // the S^T accumulators by an 8x8 transpose.  The MMA row r of a block of 8 is token tile_row(r), an
 // order in which every 16-byte shared load of K and of V is free of bank conflicts.
-// q is bf16 times an exact power of two per head, f16 (its elements below 2^-25 of the largest lose
+// q is bf16 times an exact power of two per head, f16 (its elements below 2^-27 of the largest lose
 // bits).  With lv = log2 vs of the tile, the weights enter the second product as
 // f16(2^(15 + s + lv - M)), M the running maximum of s + lv, and the sum as fp32 2^(s - m).  f16
 // because it is what the MMA takes beside the cache's exact f16 values; 2^15 because half of its range

@@ -427,6 +427,22 @@ def test_decode_blocks_ranges(case):
     check_decode(q, kc, vc, ks, vs, tables, context, scale)
 
 
+@pytest.mark.parametrize("scales", ["half_zero", "all_zero", "tiny", "zero_at_the_largest_weight"])
+def test_decode_blocks_value_scales_down_to_zero(scales):
+    q, kc, vc, ks, vs, tables, context = decode_case(16, 2, 4, 256, 64, [700, 65, 30000, 129])
+    if scales == "half_zero":
+        vs[torch.rand(vs.shape, generator=torch.Generator().manual_seed(17)).to(DEV) < 0.5] = 0
+    elif scales == "all_zero":
+        vs.zero_()
+    elif scales == "tiny":
+        vs.fill_(2.0 ** -120)
+    else:  # the first group of each sequence has the largest scores by far, and no values
+        first = [row[0] for row in tables]
+        ks[first, 0] = 2.0
+        vs[first, 0] = 0
+    check_decode(q, kc, vc, ks, vs, tables, context)
+
+
 def test_decode_blocks_nan_in_a_live_row_reaches_the_output():
     q, kc, vc, ks, vs, tables, context = decode_case(13, 2, 2, 256, 64, [300, 80])
     kc.view(torch.uint8)[tables[0][1], 10, 0, 3] = 0x7F
