@@ -560,7 +560,8 @@ def paged_decode_fp8_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             workspace: torch.Tensor | None = None) -> torch.Tensor:
     """paged_decode over the cache of store_kvcache_fp8_blocks: one new token per sequence, q
     [B, Hq, D] (or [B, 1, Hq, D]) bf16, Hq / Hk <= 16; block_tables [>= B, MB] int32, context_lens
-    [>= B] int32.  Returns out [B, Hq, D].  Error bits: decode_errors(workspace)."""
+    [>= B] int32.  Returns out [B, Hq, D].  workspace (None: made and zero-filled by every call) from
+    make_block_decode_workspace.  Error bits: decode_errors(workspace)."""
     if q.dim() == 4:
         assert q.shape[1] == 1
         q = q.squeeze(1)
