@@ -746,6 +746,14 @@ def test_logprobs_where_the_forms_of_the_exponent_meet(middle):
         check_logprobs_of_any_size(x, torch.randint(0, vocab, (rows,), generator=g, device=DEV), 8)
 
 
+@pytest.mark.parametrize("rows", [1, 149, 600])
+def test_logprobs_of_large_logits_one_step_of_fp32_apart(rows):
+    """Most of a row at 2e8, some a step of 16 above it: the reference has to be the row's maximum."""
+    g = torch.Generator(device=DEV).manual_seed(65)
+    x = 2e8 + 16.0 * (torch.rand(rows, 77412, generator=g, device=DEV) < 0.0036)
+    check_logprobs_of_any_size(x, torch.randint(0, 77412, (rows,), generator=g, device=DEV), 5)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_logprobs_are_never_positive_and_entropies_never_negative(dtype):
     """Confident rows, whose own token is nearly certain."""
